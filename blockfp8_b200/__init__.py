@@ -18,6 +18,15 @@ from .gemm import (
     quantize_cuda,
 )
 from .layout import BLOCK_N, FP8_DTYPE, FP8_MAX, GROUP_K
+from .moe import moe, moe_experts
+from .mxfp4 import (
+    dequantize_mxfp4,
+    gemm_mxfp4,
+    linear_mxfp4,
+    quantize_mxfp4,
+    tile_mxfp4_scales,
+    untile_mxfp4_scales,
+)
 from .quant import quantize_activations, quantize_weights
 from .reference import dequantize_activations, dequantize_weights, error_bound, reference_gemm
 
@@ -29,16 +38,24 @@ __all__ = [
     "check_gemm_args",
     "configs",
     "dequantize_activations",
+    "dequantize_mxfp4",
     "dequantize_weights",
     "error_bound",
     "fused_configs",
     "gemm",
     "gemm_bf16",
+    "gemm_mxfp4",
     "linear",
+    "linear_mxfp4",
+    "moe",
+    "moe_experts",
     "native_available",
     "prefers_fused",
     "quantize_activations",
     "quantize_cuda",
+    "quantize_mxfp4",
     "quantize_weights",
     "reference_gemm",
+    "tile_mxfp4_scales",
+    "untile_mxfp4_scales",
 ]

@@ -78,6 +78,51 @@ class SiluMulQuantProblem(ctypes.Structure):
     ]
 
 
+class Mxfp4QuantProblem(ctypes.Structure):
+    """bfp8_mxfp4_quant_problem."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("x_type", ctypes.c_int),
+        ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("s", ctypes.c_void_p),
+        ("M", ctypes.c_int), ("K", ctypes.c_int),
+    ]
+
+
+class Mxfp4DequantProblem(ctypes.Structure):
+    """bfp8_mxfp4_dequant_problem."""
+    _fields_ = [
+        ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("s", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64), ("y_type", ctypes.c_int),
+        ("M", ctypes.c_int), ("K", ctypes.c_int),
+    ]
+
+
+class Mxfp4GemmProblem(ctypes.Structure):
+    """bfp8_mxfp4_gemm_problem."""
+    _fields_ = [
+        ("a", ctypes.c_void_p), ("lda", ctypes.c_int64), ("sa", ctypes.c_void_p),
+        ("b", ctypes.c_void_p), ("ldb", ctypes.c_int64), ("sb", ctypes.c_void_p),
+        ("c", ctypes.c_void_p), ("ldc", ctypes.c_int64),
+        ("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int), ("weights_ready", ctypes.c_int),
+    ]
+
+
+class MoeProblem(ctypes.Structure):
+    """bfp8_moe_problem."""
+    _fields_ = [
+        ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("x_type", ctypes.c_int),
+        ("logits", ctypes.c_void_p), ("ld_logits", ctypes.c_int64), ("logits_type", ctypes.c_int),
+        ("ids", ctypes.c_void_p), ("weights", ctypes.c_void_p),
+        ("renormalize", ctypes.c_int), ("format", ctypes.c_int),
+        ("w13", ctypes.c_void_p), ("w13_expert", ctypes.c_int64), ("w13_row", ctypes.c_int64),
+        ("s13", ctypes.c_void_p),
+        ("w2", ctypes.c_void_p), ("w2_expert", ctypes.c_int64), ("w2_row", ctypes.c_int64),
+        ("s2", ctypes.c_void_p),
+        ("y", ctypes.c_void_p), ("ldy", ctypes.c_int64),
+        ("T", ctypes.c_int), ("H", ctypes.c_int), ("I", ctypes.c_int), ("E", ctypes.c_int),
+        ("top_k", ctypes.c_int),
+    ]
+
+
 TP_MAX_RANKS = 8
 IPC_HANDLE_BYTES = 64
 
@@ -123,6 +168,11 @@ _SIGNATURES = {
     "bfp8_launch_quantize": ([ctypes.POINTER(QuantProblem), ctypes.c_void_p], ctypes.c_int),
     "bfp8_launch_rmsnorm_quant": ([ctypes.POINTER(RmsNormQuantProblem), ctypes.c_void_p], ctypes.c_int),
     "bfp8_launch_silu_mul_quant": ([ctypes.POINTER(SiluMulQuantProblem), ctypes.c_void_p], ctypes.c_int),
+    "bfp8_launch_mxfp4_quantize": ([ctypes.POINTER(Mxfp4QuantProblem), ctypes.c_void_p], ctypes.c_int),
+    "bfp8_launch_mxfp4_dequantize": ([ctypes.POINTER(Mxfp4DequantProblem), ctypes.c_void_p], ctypes.c_int),
+    "bfp8_launch_mxfp4_gemm": ([ctypes.POINTER(Mxfp4GemmProblem), ctypes.c_void_p], ctypes.c_int),
+    "bfp8_moe_workspace_bytes": ([ctypes.POINTER(MoeProblem)], ctypes.c_int64),
+    "bfp8_launch_moe": ([ctypes.POINTER(MoeProblem), ctypes.c_void_p, ctypes.c_void_p], ctypes.c_int),
     "bfp8_device_status": ([ctypes.c_int], ctypes.c_int64),
     "bfp8_probe_mma": ([ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_double),
                         ctypes.POINTER(ctypes.c_double)], ctypes.c_int),
@@ -211,6 +261,32 @@ def _register_fakes() -> None:
         q = x.new_empty((m, i), dtype=torch.float8_e4m3fn)
         s = x.new_empty(((i + 127) // 128, m), dtype=torch.float32).t()
         return q, s
+
+    @torch.library.register_fake("blockfp8_b200::quantize_mxfp4")
+    def _(x):
+        m, k = x.shape
+        return (x.new_empty((m, k // 2), dtype=torch.uint8),
+                x.new_empty(((m + 127) // 128, (k + 127) // 128, 32, 16), dtype=torch.uint8))
+
+    @torch.library.register_fake("blockfp8_b200::dequantize_mxfp4")
+    def _(q, scales, dtype=torch.bfloat16):
+        return q.new_empty((q.shape[0], 2 * q.shape[1]), dtype=dtype)
+
+    @torch.library.register_fake("blockfp8_b200::gemm_mxfp4")
+    def _(a, a_scales, b, b_scales):
+        return a.new_empty((a.shape[0], b.shape[0]), dtype=torch.bfloat16)
+
+    @torch.library.register_fake("blockfp8_b200::linear_mxfp4")
+    def _(x, b, b_scales):
+        return x.new_empty((x.shape[0], b.shape[0]), dtype=torch.bfloat16)
+
+    @torch.library.register_fake("blockfp8_b200::moe")
+    def _(x, router_logits, w13, w13_scales, w2, w2_scales, top_k, renormalize=True):
+        return x.new_empty(x.shape)
+
+    @torch.library.register_fake("blockfp8_b200::moe_experts")
+    def _(x, topk_ids, topk_weights, w13, w13_scales, w2, w2_scales):
+        return x.new_empty(x.shape)
 
 
 def device_status(reset: bool = False) -> int:

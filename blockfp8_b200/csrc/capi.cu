@@ -24,6 +24,9 @@
 #include <vector>
 
 #include "gemm_kernel.cuh"
+#include "moe.cuh"
+#include "mx_gemm.cuh"
+#include "mxfp4.cuh"
 #include "probes.cuh"
 #include "producers.cuh"
 #include "quantize.cuh"
@@ -1180,6 +1183,8 @@ int64_t bfp8_device_status(int reset) {
 }
 
 }  // extern "C"
+
+#include "experts_host.cuh"
 
 // ---- roofline probes (no reference counterpart) ------------------------------------
 

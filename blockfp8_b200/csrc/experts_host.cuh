@@ -1,0 +1,350 @@
+// Host side of the MXFP4 operators and the expert layer: checks, launch
+// shapes and the C ABI (include/blockfp8_b200.h).  Included by capi.cu.
+#pragma once
+
+namespace bfp8 {
+namespace {
+
+// Raise a kernel's shared-memory limit once per device.
+int allow_smem(const void* kernel, int bytes, int dev, std::atomic<uint64_t>& done) {
+  const uint64_t bit = dev < 64 ? (uint64_t(1) << dev) : 0;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return BFP8_OK;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+  done.fetch_or(bit, std::memory_order_release);
+  return BFP8_OK;
+}
+
+int element_size(int type) { return type == 0 ? 4 : 2; }
+
+// ---- MXFP4 quantization -----------------------------------------------------------
+
+int check_codes(const void* q, int64_t ldq, const void* s, int M, int K) {
+  if (M < 0 || K <= 0 || K % 32 != 0) return fail(BFP8_EINVAL, "K must be a positive multiple of 32");
+  if (M == 0) return BFP8_OK;
+  if (!q || !s) return fail(BFP8_EINVAL, "null operand pointer");
+  if (!aligned16(q) || !aligned16(s) || ldq < K / 2 || ldq % 16 != 0)
+    return fail(BFP8_EINVAL, "codes must be row-major with 16-byte aligned rows, scales 16-byte aligned");
+  return BFP8_OK;
+}
+
+int launch_mx(const void* kernel, int m_tiles, int k_tiles, void** args, int num_sms, cudaStream_t stream,
+              const char* what) {
+  const int64_t tasks = int64_t(m_tiles) * 32 * cdiv(k_tiles, 2);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(std::min<int64_t>((tasks + kMxThreads / 32 - 1) / (kMxThreads / 32), int64_t(num_sms) * 16)));
+  cfg.blockDim = dim3(kMxThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  set_pdl(cfg, attr);
+  cudaError_t e = cudaLaunchKernelExC(&cfg, kernel, args);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, what);
+  return BFP8_OK;
+}
+
+// ---- MXFP4 GEMM -------------------------------------------------------------------
+
+template <class Cfg>
+int launch_mx_gemm(MxGemmParams& gp, const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  const void* kernel = reinterpret_cast<const void*>(&mx_gemm_kernel<Cfg>);
+  if (int r = allow_smem(kernel, Cfg::SMEM_BYTES, dev, done)) return r;
+  if (int r = make_map(&gp.map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.b, uint64_t(p.K / 2), uint64_t(p.N), uint64_t(p.ldb),
+                       128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
+    return r;
+  if (int r = make_map(&gp.map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, uint64_t(p.K / 2), uint64_t(p.M), uint64_t(p.lda),
+                       128, Cfg::BN, CU_TENSOR_MAP_SWIZZLE_128B))
+    return r;
+  gp.m_tiles = cdiv(p.M, Cfg::BN);
+  const int64_t tiles = int64_t(gp.n_tiles) * gp.m_tiles;
+  // K parts while the CTAs still fit two to an SM and each has two stages.
+  int splits = 1;
+  while (splits < 8 && tiles * splits * 2 <= 2 * int64_t(num_sms) && gp.k_stages >= splits * 4) splits *= 2;
+  gp.splits = splits;
+  if (tiles * splits > INT32_MAX) return fail(BFP8_EINVAL, "too many tiles for one launch");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(tiles * splits));
+  cfg.blockDim = dim3(Cfg::THREADS);
+  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  set_pdl(cfg, attr);
+  if (splits > 1) {
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = unsigned(splits);
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+  }
+  cudaError_t e = cudaLaunchKernelEx(&cfg, mx_gemm_kernel<Cfg>, gp);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "MXFP4 GEMM launch");
+  return BFP8_OK;
+}
+
+// ---- the expert layer ---------------------------------------------------------------
+
+struct MoeShape {
+  int nt;        // 8-token tiles of a chunk
+  int segments;  // K ranges of DOWN
+  int seg_len;
+};
+
+constexpr int kMoeMaxHidden = 8192;
+constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
+constexpr int kMoeMinStages = 3;
+
+int round_up(int x, int m) { return cdiv(x, m) * m; }
+
+struct MoeLayout {
+  int stages, stage_row, smem;
+  uint32_t off_b, off_ts, off_red, off_route, off_bars;
+};
+
+// Shared memory of one kernel whose units span k values: as many stages as
+// fit beside the activations.
+bool moe_layout(const bfp8_moe_problem& p, int k, int nt, MoeLayout* out) {
+  const int P = p.T * p.top_k, blocks = cdiv(k, 128), bb = p.format ? 64 : 128;
+  const int row = blocks * bb;                      // bytes of a unit's row
+  out->stage_row = round_up(cdiv(row, cdiv(row, 1024)), bb);
+  const int stage = 16 * (out->stage_row + 16);
+  const int b = blocks * 2048 * nt, ts = blocks * 8 * nt * 4, red = 2 * kMoeConsumers * nt * 512;
+  const int route = round_up(moe_route_bytes(P), 16);
+  const int fixed = b + ts + red + route + 16 * 8 * 2 + 64 + 16;
+  const int stages = std::min(16, (kMaxSmem - fixed) / stage);
+  if (stages < kMoeMinStages) return false;
+  const int scratch = p.E * cdiv(P, 32) * 4 + p.E * 4;
+  if (stages * stage < scratch) return false;
+  out->stages = stages;
+  out->off_b = uint32_t(round_up(stages * stage, 128));
+  out->off_ts = out->off_b + uint32_t(b);
+  out->off_red = out->off_ts + uint32_t(round_up(ts, 16));
+  out->off_route = out->off_red + uint32_t(red);
+  out->off_bars = out->off_route + uint32_t(route);
+  out->smem = int(out->off_bars) + 8 * (2 * stages + 4) + 16;
+  return out->smem <= kMaxSmem;
+}
+
+// Tokens of a chunk: 16 where the batch can fill them and the activations of
+// both kernels leave room for the ring, else 8.
+bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
+  s->segments = cdiv(p.I, kMoeSegment);
+  s->seg_len = round_up(cdiv(p.I, s->segments), 128);
+  s->segments = cdiv(p.I, s->seg_len);
+  MoeLayout lay;
+  for (s->nt = p.T > 8 ? 2 : 1; s->nt >= 1; --s->nt)
+    if (moe_layout(p, p.H, s->nt, &lay) && moe_layout(p, std::min(p.I, s->seg_len), s->nt, &lay)) return true;
+  return false;
+}
+
+int check_moe(const bfp8_moe_problem& p) {
+  if (p.T < 1 || p.T > kMoeMaxTokens) return fail(BFP8_EINVAL, "the expert layer takes 1 to 64 tokens");
+  if (p.H < 32 || p.H % 32 || p.H > kMoeMaxHidden)
+    return fail(BFP8_EINVAL, "H must be a multiple of 32, at most 8192");
+  if (p.I < 32 || p.I % 32) return fail(BFP8_EINVAL, "I must be a positive multiple of 32");
+  if (p.E < 1 || p.E > kMoeMaxExperts) return fail(BFP8_EINVAL, "1 to 512 experts");
+  if (p.top_k < 1 || p.top_k > kMoeMaxTopK || p.top_k > p.E)
+    return fail(BFP8_EINVAL, "top_k must be at least 1 and at most min(16, E)");
+  if (p.x_type != 1 && p.x_type != 2) return fail(BFP8_EINVAL, "x must be bf16 or fp16");
+  if (p.format != 0 && p.format != 1) return fail(BFP8_EINVAL, "unknown weight format");
+  if (!p.x || !p.y || !p.w13 || !p.s13 || !p.w2 || !p.s2) return fail(BFP8_EINVAL, "null operand pointer");
+  if (p.logits ? (p.ids || p.weights) : (!p.ids || !p.weights))
+    return fail(BFP8_EINVAL, "either logits, or ids and weights");
+  if (p.logits && (p.ld_logits < p.E || p.logits_type < 0 || p.logits_type > 2))
+    return fail(BFP8_EINVAL, "logits must be row-major fp32, bf16 or fp16");
+  if (!aligned16(p.x) || p.ldx < p.H || p.ldx % 8 || !aligned16(p.y) || p.ldy < p.H || p.ldy % 8)
+    return fail(BFP8_EINVAL, "x and y must be row-major with 16-byte aligned rows");
+  const int64_t k13 = p.format ? p.H / 2 : p.H, k2 = p.format ? p.I / 2 : p.I;
+  if (!aligned16(p.w13) || !aligned16(p.w2) || p.w13_row < k13 || p.w13_row % 16 || p.w2_row < k2 || p.w2_row % 16 ||
+      p.w13_expert % 16 || p.w2_expert % 16)
+    return fail(BFP8_EINVAL, "expert weights must be row-major with 16-byte aligned rows");
+  if (!aligned16(p.s13) || !aligned16(p.s2)) return fail(BFP8_EINVAL, "scales must be 16-byte aligned");
+  return BFP8_OK;
+}
+
+template <class Cfg>
+int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  if (int r = allow_smem(reinterpret_cast<const void*>(&moe_kernel<Cfg>), kMaxSmem, dev, done)) return r;
+  mp.stages = lay.stages;
+  mp.stage_row = lay.stage_row;
+  mp.off_b = lay.off_b;
+  mp.off_ts = lay.off_ts;
+  mp.off_red = lay.off_red;
+  mp.off_route = lay.off_route;
+  mp.off_bars = lay.off_bars;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(num_sms));
+  cfg.blockDim = dim3(kMoeThreads);
+  cfg.dynamicSmemBytes = size_t(lay.smem);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  set_pdl(cfg, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, moe_kernel<Cfg>, mp);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "expert layer launch");
+  return BFP8_OK;
+}
+
+template <bool GATE>
+int launch_moe_any(MoeParams& mp, const MoeLayout& lay, int format, int nt, int x_type, int dev, int num_sms,
+                   cudaStream_t stream) {
+  auto go = [&](auto mx, auto tiles, auto t) {
+    return launch_moe_kernel<MoeCfg<GATE, decltype(mx)::value, decltype(tiles)::value, decltype(t)>>(mp, lay, dev,
+                                                                                                     num_sms, stream);
+  };
+  auto by_type = [&](auto mx, auto tiles) {
+    return x_type == 1 ? go(mx, tiles, __nv_bfloat16()) : go(mx, tiles, __half());
+  };
+  auto by_tiles = [&](auto mx) {
+    return nt == 1 ? by_type(mx, std::integral_constant<int, 1>()) : by_type(mx, std::integral_constant<int, 2>());
+  };
+  return format ? by_tiles(std::true_type()) : by_tiles(std::false_type());
+}
+
+}  // namespace
+}  // namespace bfp8
+
+extern "C" {
+
+int bfp8_launch_mxfp4_quantize(const bfp8_mxfp4_quant_problem* pp, void* stream) {
+  if (!pp) return fail(BFP8_EINVAL, "null problem");
+  const bfp8_mxfp4_quant_problem& p = *pp;
+  if (p.x_type < 0 || p.x_type > 2) return fail(BFP8_EINVAL, "x must be fp32, bf16 or fp16");
+  if (int r = check_codes(p.q, p.ldq, p.s, p.M, p.K)) return r;
+  if (p.M == 0) return BFP8_OK;
+  if (!p.x || !aligned16(p.x) || p.ldx < p.K || (p.ldx * element_size(p.x_type)) % 16)
+    return fail(BFP8_EINVAL, "x must be row-major with 16-byte aligned rows");
+  int dev = 0;
+  const int num_sms = current_device_sms(&dev);
+  if (num_sms < 0) return num_sms;
+  Mxfp4QuantParams k{p.x, p.ldx, static_cast<uint8_t*>(p.q), p.ldq, static_cast<uint8_t*>(p.s), p.M, p.K,
+                     cdiv(p.M, 128), cdiv(p.K, 128)};
+  void* args[] = {&k};
+  const void* kernel = p.x_type == 0   ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<float>)
+                       : p.x_type == 1 ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<__nv_bfloat16>)
+                                       : reinterpret_cast<const void*>(&mxfp4_quantize_kernel<__half>);
+  return launch_mx(kernel, k.m_tiles, k.k_tiles, args, num_sms, static_cast<cudaStream_t>(stream),
+                   "MXFP4 quantization launch");
+}
+
+int bfp8_launch_mxfp4_dequantize(const bfp8_mxfp4_dequant_problem* pp, void* stream) {
+  if (!pp) return fail(BFP8_EINVAL, "null problem");
+  const bfp8_mxfp4_dequant_problem& p = *pp;
+  if (p.y_type < 0 || p.y_type > 1) return fail(BFP8_EINVAL, "y must be fp32 or bf16");
+  if (int r = check_codes(p.q, p.ldq, p.s, p.M, p.K)) return r;
+  if (p.M == 0) return BFP8_OK;
+  if (!p.y || !aligned16(p.y) || p.ldy < p.K || (p.ldy * element_size(p.y_type)) % 16)
+    return fail(BFP8_EINVAL, "y must be row-major with 16-byte aligned rows");
+  int dev = 0;
+  const int num_sms = current_device_sms(&dev);
+  if (num_sms < 0) return num_sms;
+  Mxfp4DequantParams k{static_cast<const uint8_t*>(p.q), p.ldq, static_cast<const uint8_t*>(p.s), p.y, p.ldy, p.M, p.K,
+                       cdiv(p.M, 128), cdiv(p.K, 128)};
+  void* args[] = {&k};
+  const void* kernel = p.y_type == 0 ? reinterpret_cast<const void*>(&mxfp4_dequantize_kernel<float>)
+                                     : reinterpret_cast<const void*>(&mxfp4_dequantize_kernel<__nv_bfloat16>);
+  return launch_mx(kernel, k.m_tiles, k.k_tiles, args, num_sms, static_cast<cudaStream_t>(stream),
+                   "MXFP4 dequantization launch");
+}
+
+int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* pp, void* stream) {
+  if (!pp) return fail(BFP8_EINVAL, "null problem");
+  const bfp8_mxfp4_gemm_problem& p = *pp;
+  if (p.N <= 0 || p.N % 8) return fail(BFP8_EINVAL, "N must be a positive multiple of 8");
+  if (int r = check_codes(p.a, p.lda, p.sa, p.M, p.K)) return r;
+  if (p.M == 0) return BFP8_OK;
+  if (int r = check_codes(p.b, p.ldb, p.sb, p.N, p.K)) return r;
+  if (!p.c || !aligned16(p.c) || p.ldc < p.N || p.ldc % 8)
+    return fail(BFP8_EINVAL, "c must be row-major with 8-element aligned rows");
+  int dev = 0;
+  const int num_sms = current_device_sms(&dev);
+  if (num_sms < 0) return num_sms;
+  MxGemmParams gp;
+  std::memset(&gp, 0, sizeof(gp));
+  gp.sw = static_cast<const uint8_t*>(p.sb);
+  gp.sx = static_cast<const uint8_t*>(p.sa);
+  gp.c = static_cast<__nv_bfloat16*>(p.c);
+  gp.ldc = p.ldc;
+  gp.M = p.M;
+  gp.N = p.N;
+  gp.K = p.K;
+  gp.n_tiles = cdiv(p.N, 128);
+  gp.k_tiles = cdiv(p.K, 128);
+  gp.k_stages = cdiv(p.K, 256);
+  gp.early = p.weights_ready ? 1 : 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.M <= 16) return launch_mx_gemm<MxCfg<16, 5>>(gp, p, dev, num_sms, s);
+  if (p.M <= 32) return launch_mx_gemm<MxCfg<32, 5>>(gp, p, dev, num_sms, s);
+  if (p.M <= 64) return launch_mx_gemm<MxCfg<64, 4>>(gp, p, dev, num_sms, s);
+  return launch_mx_gemm<MxCfg<128, 3>>(gp, p, dev, num_sms, s);
+}
+
+int64_t bfp8_moe_workspace_bytes(const bfp8_moe_problem* pp) {
+  if (!pp) return fail(BFP8_EINVAL, "null problem");
+  const bfp8_moe_problem& p = *pp;
+  if (int r = check_moe(p)) return r;
+  MoeShape s;
+  if (!moe_shape(p, &s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
+  const int64_t pairs = int64_t(p.T) * p.top_k;
+  return align256(pairs * p.I * 4) + align256(pairs * s.segments * p.H * 4) + align256(int64_t(p.H) / 16 * 4);
+}
+
+int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
+  if (!pp) return fail(BFP8_EINVAL, "null problem");
+  const bfp8_moe_problem& p = *pp;
+  if (int r = check_moe(p)) return r;
+  if (!workspace || !aligned16(workspace)) return fail(BFP8_EINVAL, "the workspace must be 16-byte aligned");
+  MoeShape s;
+  if (!moe_shape(p, &s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
+  int dev = 0;
+  const int num_sms = current_device_sms(&dev);
+  if (num_sms < 0) return num_sms;
+  const int64_t pairs = int64_t(p.T) * p.top_k;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  MoeParams mp;
+  std::memset(&mp, 0, sizeof(mp));
+  mp.x = p.x;
+  mp.ldx = p.ldx;
+  mp.logits = p.logits;
+  mp.ld_logits = p.ld_logits;
+  mp.logits_type = p.logits_type;
+  mp.ids = p.ids;
+  mp.weights = p.weights;
+  mp.renormalize = p.renormalize;
+  mp.h = reinterpret_cast<float*>(ws);
+  mp.z = reinterpret_cast<float*>(ws + align256(pairs * p.I * 4));
+  mp.counters = reinterpret_cast<int*>(ws + align256(pairs * p.I * 4) + align256(pairs * s.segments * p.H * 4));
+  mp.y = p.y;
+  mp.ldy = p.ldy;
+  mp.T = p.T;
+  mp.H = p.H;
+  mp.I = p.I;
+  mp.E = p.E;
+  mp.top_k = p.top_k;
+  MoeLayout lay;
+  moe_layout(p, p.H, s.nt, &lay);
+  mp.w = static_cast<const uint8_t*>(p.w13);
+  mp.w_expert = p.w13_expert;
+  mp.w_row = p.w13_row;
+  mp.ws = p.s13;
+  mp.rb = cdiv(2 * p.I, 128);
+  mp.kb = cdiv(p.H, 128);
+  mp.segments = 1;
+  mp.seg_len = round_up(p.H, 128);
+  if (int r = launch_moe_any<true>(mp, lay, p.format, s.nt, p.x_type, dev, num_sms, static_cast<cudaStream_t>(stream)))
+    return r;
+  moe_layout(p, std::min(p.I, s.seg_len), s.nt, &lay);
+  mp.w = static_cast<const uint8_t*>(p.w2);
+  mp.w_expert = p.w2_expert;
+  mp.w_row = p.w2_row;
+  mp.ws = p.s2;
+  mp.rb = cdiv(p.H, 128);
+  mp.kb = cdiv(p.I, 128);
+  mp.segments = s.segments;
+  mp.seg_len = s.seg_len;
+  return launch_moe_any<false>(mp, lay, p.format, s.nt, p.x_type, dev, num_sms, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

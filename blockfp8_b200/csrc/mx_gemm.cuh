@@ -1,0 +1,232 @@
+// MXFP4 GEMM on the block-scaled tensor cores (tcgen05.mma.kind::mxf4):
+//
+//   C[m, n] = sum_b 2^(ea[m, b] + eb[n, b]) sum_{k in block b of 32} A[m, k] B[n, k]
+//
+// The scales go into tensor memory beside the accumulator and the MMA applies
+// them, so there is no promotion step between K blocks: a tile's whole K
+// range accumulates in fp32 in TMEM, and the epilogue rounds once to bf16.
+//
+// The 128 MMA rows are weight rows and the BN columns are tokens (BN = 16 to
+// 128), so a decode batch pays for no padding rows.  One CTA per (tile, K
+// part): a cluster of up to 8 CTAs along K splits a tile's K range where there
+// are few tiles, and its CTAs sum their parts over distributed shared memory,
+// always in rank order -- no workspace, no counters, nothing shared between
+// launches.  Two CTAs fit on an SM, so one's epilogue overlaps another's loop.
+//
+// Stages of K = 256: 128 bytes of codes per row (one 128-byte-swizzled TMA
+// box for the weights, one for the tokens) and 512 bytes of scales per 128
+// rows per 128 of K (bulk copies; the scale layout is the order in which
+// tcgen05.cp wants them).  Per stage one thread issues the scale copies to
+// TMEM and four MMAs of K = 64; tcgen05 runs them in order.
+//
+// Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-5 epilogue.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+
+#include <cstdint>
+
+#include "ptx.cuh"
+
+namespace bfp8 {
+
+struct MxGemmParams {
+  CUtensorMap map_w;  // weight codes [N, K / 2] bytes: [128 x 128] boxes, 128-byte swizzle
+  CUtensorMap map_x;  // token codes [M, K / 2] bytes: [BN x 128] boxes
+  const uint8_t* sw;  // weight scales [ceil(N / 128), k_tiles, 512]
+  const uint8_t* sx;  // token scales [ceil(M / 128), k_tiles, 512]
+  __nv_bfloat16* c;   // [M, N], row stride ldc
+  int64_t ldc;
+  int M, N, K;
+  int n_tiles;   // weight tiles (128 rows)
+  int m_tiles;   // token tiles (BN)
+  int k_tiles;   // 128-wide scale tiles
+  int k_stages;  // 256-wide stages
+  int splits;    // CTAs of a cluster along K
+  int early;     // weights may be requested before griddepcontrol.wait
+};
+
+enum MxWaitSite : uint32_t {
+  kMxWaitEmpty = 33,
+  kMxWaitFull = 34,
+  kMxWaitDone = 35,
+  kMxWaitDrain = 36,
+};
+
+template <int BN_, int STAGES_>
+struct MxCfg {
+  static constexpr int BN = BN_, STAGES = STAGES_;
+  static constexpr int THREADS = 192;
+  static constexpr int W_BYTES = 128 * 128, X_BYTES = BN * 128, S_BYTES = 1024;  // per stage
+  static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + 2 * S_BYTES;
+  static constexpr int ACC_COLS = BN < 32 ? 32 : BN;
+  // two stages' scales: 2 K tiles x (4 weight + 4 token) columns each
+  static constexpr int TMEM_COLS = BN <= 32 ? 64 : (BN == 64 ? 128 : 256);
+  static_assert(ACC_COLS + 32 <= TMEM_COLS, "TMEM");
+  static constexpr int RING = STAGES * STAGE_BYTES;
+  static_assert(RING >= 128 * BN * 4, "the ring holds the tile's fp32 sums at the end");
+  static constexpr int SMEM_BYTES = 1024 + RING + (2 * STAGES + 1) * 8 + 16;
+};
+
+template <class Cfg>
+__global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_constant__ MxGemmParams p) {
+  constexpr int BN = Cfg::BN, S = Cfg::STAGES;
+  griddep_launch_dependents();
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  auto w_tile = [&](int s) { return base + uint32_t(s * Cfg::STAGE_BYTES); };
+  auto x_tile = [&](int s) { return w_tile(s) + Cfg::W_BYTES; };
+  auto sw_tile = [&](int s) { return x_tile(s) + Cfg::X_BYTES; };
+  auto sx_tile = [&](int s) { return sw_tile(s) + Cfg::S_BYTES; };
+  const uint32_t bars = base + Cfg::RING;
+  auto full = [&](int s) { return bars + 8u * uint32_t(s); };
+  auto empty = [&](int s) { return bars + 8u * uint32_t(S + s); };
+  const uint32_t done = bars + 8u * uint32_t(2 * S);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::RING + 8 * (2 * S + 1));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = p.splits > 1 ? int(cluster_rank()) : 0;
+  const int tile = int(blockIdx.x) / p.splits;
+  const int nt = tile % p.n_tiles, mt = tile / p.n_tiles;
+  // this CTA's stages of the tile's K range
+  const int s0 = p.k_stages * rank / p.splits, s1 = p.k_stages * (rank + 1) / p.splits;
+  const int L = s1 - s0;
+
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < 2 * S + 1; ++i) mbar_init(bars + 8u * uint32_t(i), 1u);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&p.map_w);
+    tma_prefetch_desc(&p.map_x);
+  }
+  if (warp == 1) {
+    tmem_alloc<1>(smem_u32(misc), Cfg::TMEM_COLS);
+    tmem_relinquish<1>();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol_w = p.m_tiles > 1 ? policy_evict_normal() : policy_evict_first();
+      const uint64_t pol_x = policy_evict_last();
+      auto kts = [&](int i) { return min(2, p.k_tiles - 2 * (s0 + i)); };  // scale tiles of stage i
+      auto load_w = [&](int i) {
+        const int s = i % S, k = s0 + i;
+        mbar_arrive_expect_tx(full(s), uint32_t(Cfg::W_BYTES + Cfg::X_BYTES + 2 * 512 * kts(i)));
+        tma_load_2d(w_tile(s), &p.map_w, k * 128, nt * 128, full(s), pol_w);
+        bulk_load(sw_tile(s), p.sw + (int64_t(nt) * p.k_tiles + 2 * k) * 512, uint32_t(512 * kts(i)), full(s), pol_w);
+      };
+      auto load_x = [&](int i) {
+        const int s = i % S, k = s0 + i;
+        tma_load_2d(x_tile(s), &p.map_x, k * 128, mt * BN, full(s), pol_x);
+        bulk_load(sx_tile(s), p.sx + (int64_t(mt * BN / 128) * p.k_tiles + 2 * k) * 512, uint32_t(512 * kts(i)),
+                  full(s), pol_x);
+      };
+      int pre = 0;
+      if (p.early)
+        for (; pre < S && pre < L; ++pre) load_w(pre);
+      griddep_wait();
+      for (int i = 0; i < pre; ++i) load_x(i);
+      int issued = pre;
+      for (int i = pre; i < L; ++i) {
+        if (i >= S && !mbar_wait(empty(i % S), uint32_t(i / S - 1) & 1u, abort_flag, kMxWaitEmpty)) break;
+        load_w(i);
+        load_x(i);
+        ++issued;
+      }
+      for (int i = issued - S > 0 ? issued - S : 0; i < issued; ++i)
+        mbar_wait(full(i % S), uint32_t(i / S) & 1u, nullptr, kMxWaitDrain);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_mxf4(128, BN);
+      const uint32_t scales = tmem + Cfg::ACC_COLS;
+      for (int i = 0; i < L; ++i) {
+        const int s = i % S;
+        if (!mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull)) break;
+        tc_fence_after();
+        const int left = p.K - (s0 + i) * 256;  // values of K from this stage on
+        const int steps = left >= 256 ? 4 : (left + 63) / 64;
+        const uint32_t sf = scales + uint32_t(16 * (i & 1));  // [kt][4 weight + 4 token] columns
+        for (int kt = 0; kt < (steps + 1) / 2; ++kt) {
+          tmem_cp_scales(sf + uint32_t(8 * kt), smem_desc_scales(sw_tile(s) + uint32_t(512 * kt)));
+          tmem_cp_scales(sf + uint32_t(8 * kt + 4), smem_desc_scales(sx_tile(s) + uint32_t(512 * kt)));
+        }
+        const uint64_t a = smem_desc_k128_sw128(w_tile(s)), b = smem_desc_k128_sw128(x_tile(s));
+#pragma unroll
+        for (int k = 0; k < 4; ++k)  // K = 64 codes = 32 bytes = 2 descriptor units
+          if (k < steps)
+            mma_mxf4<1>(tmem, a + 2 * k, b + 2 * k, idesc | idesc_scale_half(k & 1), sf + uint32_t(8 * (k >> 1)),
+                        sf + uint32_t(8 * (k >> 1) + 4), (i > 0 || k > 0) ? 1u : 0u);
+        mma_commit<1>(empty(s));
+      }
+      mma_commit<1>(done);
+      mbar_wait(done, 0, nullptr, kMxWaitDone);
+    }
+    __syncwarp();
+  }
+  // Every load has landed and every MMA is done: the ring is free.
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+
+  // Sums to shared memory, [token][weight row] fp32: lanes hold consecutive rows.
+  float* sums = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    const int q = warp & 3;  // the TMEM lanes this warp may read
+    const int row = 32 * q + lane;
+    const uint32_t t_lane = tmem + (uint32_t(32 * q) << 16);
+#pragma unroll 1
+    for (int c = 0; c < BN; c += 16) {
+      float v[16];
+      tmem_ld16(t_lane + uint32_t(c), v);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + row] = L > 0 ? v[j] : 0.f;
+    }
+  }
+  tc_fence_before();
+  if (p.splits > 1) cluster_sync();
+  else __syncthreads();
+  tc_fence_after();
+
+  // This CTA's share of the tile's tokens: two weight rows a thread, the parts
+  // in rank order.
+  {
+    griddep_wait();
+    const int c0 = BN * rank / p.splits, c1 = BN * (rank + 1) / p.splits;
+    const bool ok = !*abort_flag;
+    for (int idx = threadIdx.x; idx < (c1 - c0) * 64; idx += Cfg::THREADS) {
+      const int col = c0 + idx / 64, r2 = (idx & 63) * 2;
+      const int m = mt * BN + col, n = nt * 128 + r2;
+      if (m >= p.M || n >= p.N) continue;
+      float2 v = make_float2(0.f, 0.f);
+      if (p.splits == 1) {
+        v = *reinterpret_cast<const float2*>(sums + col * 128 + r2);
+      } else {
+        for (int r = 0; r < p.splits; ++r) {
+          const float2 w = ld_cluster_f32x2(map_shared_rank(base + uint32_t((col * 128 + r2) * 4), uint32_t(r)));
+          v.x += w.x;
+          v.y += w.y;
+        }
+      }
+      if (ok) *reinterpret_cast<__nv_bfloat162*>(p.c + int64_t(m) * p.ldc + n) = __floats2bfloat162_rn(v.x, v.y);
+    }
+  }
+  // A CTA's sums stay until every CTA of the cluster has read them.
+  if (p.splits > 1) cluster_sync();
+  else __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+}  // namespace bfp8

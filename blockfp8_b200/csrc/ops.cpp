@@ -337,15 +337,275 @@ std::tuple<at::Tensor, at::Tensor> silu_mul_quant(const at::Tensor& x, double ep
   return {q, s};
 }
 
+// ---- MXFP4 and the expert layer (torch.ops.blockfp8_b200) -------------------------
+// Every argument is checked here, once; refusals are ValueErrors.  The
+// operators are registered for CPU tensors too, so that a call on them is
+// refused with its reason (shapes and types first, then the device) rather
+// than by the dispatcher.
+
+#define CHECK_VALUE(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
+
+int float_type(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return 0;
+    case at::kBFloat16: return 1;
+    case at::kHalf: return 2;
+    default: return -1;
+  }
+}
+
+bool aligned_rows(const at::Tensor& t) {  // 2-D, contiguous 16-byte aligned rows
+  return t.stride(1) == 1 && (t.size(0) <= 1 || t.stride(0) >= t.size(1)) &&
+         (t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0) && aligned16(t);
+}
+
+// The row stride handed to the kernels; a single row's says nothing.
+int64_t row_stride(const at::Tensor& t) {
+  const int64_t unit = 16 / t.element_size();
+  return t.size(-2) > 1 ? t.stride(-2) : cdiv(t.size(-1), unit) * unit;
+}
+
+void check_mxfp4(const at::Tensor& q, const at::Tensor& s, const char* op, const char* name) {
+  CHECK_VALUE(q.scalar_type() == at::kByte && q.dim() == 2, op, ": ", name, " must be 2-D uint8 codes [rows, K / 2]");
+  const int64_t rows = q.size(0), K = 2 * q.size(1);
+  CHECK_VALUE(K > 0 && K % 32 == 0, op, ": K must be a positive multiple of 32, got ", K);
+  CHECK_VALUE(rows <= INT32_MAX / 2 && K <= INT32_MAX / 2, op, ": too large");
+  CHECK_VALUE(aligned_rows(q), op, ": ", name, " must be row-major with 16-byte aligned rows");
+  CHECK_VALUE(s.scalar_type() == at::kByte && s.dim() == 4 && s.size(0) == cdiv(rows, 128) && s.size(1) == cdiv(K, 128) &&
+                  s.size(2) == 32 && s.size(3) == 16,
+              op, ": the scales of ", name, " must be uint8 [", cdiv(rows, 128), ", ", cdiv(K, 128),
+              ", 32, 16] (tile_mxfp4_scales), got ", s.sizes());
+  CHECK_VALUE(s.is_contiguous() && aligned16(s), op, ": the scales of ", name, " must be contiguous");
+}
+
+void check_cuda(std::initializer_list<const at::Tensor*> tensors, const char* op) {
+  const at::Tensor& first = **tensors.begin();
+  for (const at::Tensor* t : tensors) {
+    CHECK_VALUE(t->device() == first.device(), op, ": all operands must be on one device");
+    CHECK_VALUE(t->is_cuda(), op, ": runs on CUDA tensors only");
+  }
+}
+
+std::tuple<at::Tensor, at::Tensor> empty_mxfp4(const at::Tensor& like, int64_t rows, int64_t K) {
+  const auto bytes = like.options().dtype(at::kByte);
+  return {at::empty({rows, K / 2}, bytes), at::empty({cdiv(rows, 128), cdiv(K, 128), 32, 16}, bytes)};
+}
+
+void check_mxfp4_input(const at::Tensor& x, const char* op) {
+  CHECK_VALUE(x.dim() == 2, op, ": x must be 2-D [M, K], got shape ", x.sizes());
+  CHECK_VALUE(x.size(1) > 0 && x.size(1) % 32 == 0, op, ": K must be a positive multiple of 32, got ", x.size(1));
+  CHECK_VALUE(x.size(0) <= INT32_MAX / 2 && x.size(1) <= INT32_MAX / 2, op, ": too large");
+  CHECK_VALUE(aligned_rows(x), op, ": x must be row-major with 16-byte aligned rows, got strides ", x.strides());
+}
+
+void launch_mxfp4_quantize(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s) {
+  const bfp8_mxfp4_quant_problem p{x.data_ptr(), row_stride(x),  float_type(x),     q.data_ptr(),
+                                   row_stride(q), s.data_ptr(), int(x.size(0)), int(x.size(1))};
+  require_abi(bfp8_launch_mxfp4_quantize(&p, at::cuda::getCurrentCUDAStream().stream()));
+}
+
+// x [M, K] -> (codes [M, K / 2], scale tiles).
+std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x) {
+  const char* op = "blockfp8_b200.quantize_mxfp4";
+  CHECK_VALUE(float_type(x) >= 0, op, ": x must be bfloat16, float16 or float32, got ", x.scalar_type());
+  check_mxfp4_input(x, op);
+  check_cuda({&x}, op);
+  const at::cuda::CUDAGuard guard(x.device());
+  auto out = empty_mxfp4(x, x.size(0), x.size(1));
+  if (x.size(0) > 0) launch_mxfp4_quantize(x, std::get<0>(out), std::get<1>(out));
+  return out;
+}
+
+at::Tensor dequantize_mxfp4(const at::Tensor& q, const at::Tensor& s, at::ScalarType dtype) {
+  const char* op = "blockfp8_b200.dequantize_mxfp4";
+  check_mxfp4(q, s, op, "q");
+  CHECK_VALUE(dtype == at::kBFloat16 || dtype == at::kFloat, op, ": dtype must be bfloat16 or float32, got ", dtype);
+  check_cuda({&q, &s}, op);
+  const at::cuda::CUDAGuard guard(q.device());
+  at::Tensor y = at::empty({q.size(0), 2 * q.size(1)}, q.options().dtype(dtype));
+  if (y.size(0) == 0) return y;
+  const bfp8_mxfp4_dequant_problem p{q.data_ptr(), row_stride(q),  s.data_ptr(), y.data_ptr(), y.stride(0),
+                                     float_type(y), int(y.size(0)), int(y.size(1))};
+  require_abi(bfp8_launch_mxfp4_dequantize(&p, at::cuda::getCurrentCUDAStream().stream()));
+  return y;
+}
+
+at::Tensor launch_mxfp4_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
+                             bool weights_ready) {
+  at::Tensor c = at::empty({a.size(0), b.size(0)}, a.options().dtype(at::kBFloat16));
+  const bfp8_mxfp4_gemm_problem p{a.data_ptr(),   row_stride(a),  sa.data_ptr(),   b.data_ptr(),
+                                  row_stride(b),  sb.data_ptr(),  c.data_ptr(),    c.stride(0),
+                                  int(a.size(0)), int(b.size(0)), int(2 * a.size(1)), weights_ready ? 1 : 0};
+  require_abi(bfp8_launch_mxfp4_gemm(&p, at::cuda::getCurrentCUDAStream().stream()));
+  return c;
+}
+
+void check_mxfp4_weights(const at::Tensor& b, const at::Tensor& b_scales, int64_t K, const char* op) {
+  check_mxfp4(b, b_scales, op, "b_q");
+  CHECK_VALUE(2 * b.size(1) == K, op, ": K mismatch: ", K, " and ", 2 * b.size(1));
+  CHECK_VALUE(b.size(0) > 0 && b.size(0) % 8 == 0, op, ": N must be a positive multiple of 8, got ", b.size(0));
+}
+
+at::Tensor gemm_mxfp4(const at::Tensor& a, const at::Tensor& a_scales, const at::Tensor& b, const at::Tensor& b_scales) {
+  const char* op = "blockfp8_b200.gemm_mxfp4";
+  check_mxfp4(a, a_scales, op, "a_q");
+  check_mxfp4_weights(b, b_scales, 2 * a.size(1), op);
+  check_cuda({&a, &a_scales, &b, &b_scales}, op);
+  const at::cuda::CUDAGuard guard(a.device());
+  if (a.size(0) == 0) return at::empty({0, b.size(0)}, a.options().dtype(at::kBFloat16));
+  // b may have been written by the kernel right before this one
+  return launch_mxfp4_gemm(a, a_scales, b, b_scales, false);
+}
+
+// quantize_mxfp4 then gemm_mxfp4.  The GEMM may request its weights while the
+// quantization kernel runs, which starts (and lets the GEMM start) only after
+// every earlier kernel has finished.
+at::Tensor linear_mxfp4(const at::Tensor& x, const at::Tensor& b, const at::Tensor& b_scales) {
+  const char* op = "blockfp8_b200.linear_mxfp4";
+  CHECK_VALUE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, op,
+              ": x must be bfloat16 or float16, got ", x.scalar_type());
+  check_mxfp4_input(x, op);
+  check_mxfp4_weights(b, b_scales, x.size(1), op);
+  check_cuda({&x, &b, &b_scales}, op);
+  const at::cuda::CUDAGuard guard(x.device());
+  if (x.size(0) == 0) return at::empty({0, b.size(0)}, x.options().dtype(at::kBFloat16));
+  const auto [q, s] = empty_mxfp4(x, x.size(0), x.size(1));
+  launch_mxfp4_quantize(x, q, s);
+  return launch_mxfp4_gemm(q, s, b, b_scales, true);
+}
+
+// One of the layer's two weight stacks: [E, rows, K] in either format.
+void check_experts(const at::Tensor& w, const at::Tensor& s, int64_t E, int64_t rows, int64_t K, bool mx, const char* op,
+                   const char* name) {
+  const int64_t cols = mx ? K / 2 : K;
+  CHECK_VALUE(w.dim() == 3 && w.size(0) == E && w.size(1) == rows && w.size(2) == cols, op, ": ", name, " must be [", E, ", ", rows, ", ",
+              cols, "], got ", w.sizes());
+  CHECK_VALUE(w.stride(2) == 1 && w.stride(1) >= cols && w.stride(1) % 16 == 0 && w.stride(0) % 16 == 0 && aligned16(w),
+              op, ": ", name, " must have contiguous, 16-byte aligned rows, got strides ", w.strides());
+  if (mx) {
+    CHECK_VALUE(s.scalar_type() == at::kByte && s.dim() == 5 && s.size(0) == E && s.size(1) == cdiv(rows, 128) &&
+                    s.size(2) == cdiv(K, 128) && s.size(3) == 32 && s.size(4) == 16,
+                op, ": the scales of ", name, " must be uint8 [", E, ", ", cdiv(rows, 128), ", ", cdiv(K, 128),
+                ", 32, 16] (tile_mxfp4_scales), got ", s.sizes());
+  } else {
+    CHECK_VALUE(s.scalar_type() == at::kFloat && s.dim() == 3 && s.size(0) == E && s.size(1) == cdiv(rows, 128) &&
+                    s.size(2) == cdiv(K, 128),
+                op, ": the scales of ", name, " must be float32 [", E, ", ", cdiv(rows, 128), ", ", cdiv(K, 128), "], got ",
+                s.sizes());
+  }
+  CHECK_VALUE(s.is_contiguous() && aligned16(s), op, ": the scales of ", name, " must be contiguous");
+}
+
+at::Tensor launch_moe(const char* op, const at::Tensor& x, const at::Tensor& w13, const at::Tensor& w13_scales,
+                      const at::Tensor& w2, const at::Tensor& w2_scales, int64_t E, int64_t top_k,
+                      bfp8_moe_problem p, std::initializer_list<const at::Tensor*> all) {
+  CHECK_VALUE(x.dim() == 2 && (x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf), op,
+              ": x must be 2-D bfloat16 or float16 [T, H]");
+  const int64_t T = x.size(0), H = x.size(1);
+  CHECK_VALUE(T <= 64, op, ": at most 64 tokens, got ", T);
+  CHECK_VALUE(H >= 32 && H % 32 == 0 && H <= 8192, op, ": H must be a multiple of 32, at most 8192, got ", H);
+  CHECK_VALUE(aligned_rows(x), op, ": x must be row-major with 16-byte aligned rows, got strides ", x.strides());
+  CHECK_VALUE(E >= 1 && E <= 512, op, ": 1 to 512 experts, got ", E);
+  CHECK_VALUE(top_k >= 1 && top_k <= std::min<int64_t>(16, E), op, ": top_k must be at least 1 and at most min(16, E), got ",
+              top_k);
+  const bool mx = w13.scalar_type() == at::kByte;
+  CHECK_VALUE(w2.dim() == 3 && w2.scalar_type() == w13.scalar_type() && (mx || w13.scalar_type() == at::kFloat8_e4m3fn), op,
+              ": w13 and w2 must both be float8_e4m3fn [E, rows, K] or both uint8 MXFP4 codes [E, rows, K / 2]");
+  const int64_t I = w2.size(2) * (mx ? 2 : 1);
+  CHECK_VALUE(I >= 32 && I % 32 == 0 && I <= (1 << 24), op, ": I must be a positive multiple of 32, got ", I);
+  check_experts(w13, w13_scales, E, 2 * I, H, mx, op, "w13");
+  check_experts(w2, w2_scales, E, H, I, mx, op, "w2");
+  check_cuda(all, op);
+  const at::cuda::CUDAGuard guard(x.device());
+  at::Tensor y = at::empty({T, H}, x.options());
+  if (T == 0) return y;
+  p.x = x.data_ptr();
+  p.ldx = row_stride(x);
+  p.x_type = float_type(x);
+  p.format = mx ? 1 : 0;
+  p.w13 = w13.data_ptr();
+  p.w13_expert = w13.stride(0);
+  p.w13_row = w13.stride(1);
+  p.s13 = w13_scales.data_ptr();
+  p.w2 = w2.data_ptr();
+  p.w2_expert = w2.stride(0);
+  p.w2_row = w2.stride(1);
+  p.s2 = w2_scales.data_ptr();
+  p.y = y.data_ptr();
+  p.ldy = y.stride(0);
+  p.T = int(T);
+  p.H = int(H);
+  p.I = int(I);
+  p.E = int(E);
+  p.top_k = int(top_k);
+  const int64_t bytes = bfp8_moe_workspace_bytes(&p);
+  require_abi(int(std::min<int64_t>(bytes, 0)));
+  const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
+  require_abi(bfp8_launch_moe(&p, ws.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
+  return y;
+}
+
+at::Tensor moe(const at::Tensor& x, const at::Tensor& router_logits, const at::Tensor& w13, const at::Tensor& w13_scales,
+               const at::Tensor& w2, const at::Tensor& w2_scales, int64_t top_k, bool renormalize) {
+  const char* op = "blockfp8_b200.moe";
+  CHECK_VALUE(router_logits.dim() == 2 && float_type(router_logits) >= 0 && x.dim() == 2 &&
+                  router_logits.size(0) == x.size(0) && router_logits.stride(1) == 1 &&
+                  (x.size(0) <= 1 || router_logits.stride(0) >= router_logits.size(1)),
+              op, ": router_logits must be row-major float32, bfloat16 or float16 [T, E]");
+  bfp8_moe_problem p{};
+  p.logits = router_logits.data_ptr();
+  p.ld_logits = x.size(0) > 1 ? router_logits.stride(0) : router_logits.size(1);
+  p.logits_type = float_type(router_logits);
+  p.renormalize = renormalize ? 1 : 0;
+  return launch_moe(op, x, w13, w13_scales, w2, w2_scales, router_logits.size(1), top_k, p,
+                    {&x, &router_logits, &w13, &w13_scales, &w2, &w2_scales});
+}
+
+at::Tensor moe_experts(const at::Tensor& x, const at::Tensor& topk_ids, const at::Tensor& topk_weights,
+                       const at::Tensor& w13, const at::Tensor& w13_scales, const at::Tensor& w2,
+                       const at::Tensor& w2_scales) {
+  const char* op = "blockfp8_b200.moe_experts";
+  CHECK_VALUE(topk_ids.dim() == 2 && topk_ids.scalar_type() == at::kInt && topk_weights.scalar_type() == at::kFloat &&
+                  topk_weights.sizes() == topk_ids.sizes() && x.dim() == 2 && topk_ids.size(0) == x.size(0) &&
+                  topk_ids.is_contiguous() && topk_weights.is_contiguous(),
+              op, ": topk_ids must be contiguous int32 [T, top_k] and topk_weights contiguous float32 of the same shape");
+  CHECK_VALUE(w13.dim() == 3, op, ": w13 must be 3-D");
+  bfp8_moe_problem p{};
+  p.ids = topk_ids.data_ptr<int>();
+  p.weights = topk_weights.data_ptr<float>();
+  return launch_moe(op, x, w13, w13_scales, w2, w2_scales, w13.size(0), topk_ids.size(1), p,
+                    {&x, &topk_ids, &topk_weights, &w13, &w13_scales, &w2, &w2_scales});
+}
+
 }  // namespace
 
 TORCH_LIBRARY(blockfp8_b200, m) {
+  m.def("quantize_mxfp4(Tensor x) -> (Tensor, Tensor)");
+  m.def("dequantize_mxfp4(Tensor q, Tensor scales, ScalarType dtype=bfloat16) -> Tensor");
+  m.def("gemm_mxfp4(Tensor a, Tensor a_scales, Tensor b, Tensor b_scales) -> Tensor");
+  m.def("linear_mxfp4(Tensor x, Tensor b, Tensor b_scales) -> Tensor");
+  m.def("moe(Tensor x, Tensor router_logits, Tensor w13, Tensor w13_scales, Tensor w2, Tensor w2_scales, int top_k, "
+        "bool renormalize=True) -> Tensor");
+  m.def("moe_experts(Tensor x, Tensor topk_ids, Tensor topk_weights, Tensor w13, Tensor w13_scales, Tensor w2, "
+        "Tensor w2_scales) -> Tensor");
   m.def("rms_norm_quant(Tensor x, Tensor weight, float variance_epsilon, Tensor? residual=None, "
         "float eps=1e-10) -> (Tensor, Tensor, Tensor)");
   m.def("silu_mul_quant(Tensor x, float eps=1e-10) -> (Tensor, Tensor)");
 }
 
+void impl_experts(torch::Library& m) {
+  m.impl("quantize_mxfp4", &quantize_mxfp4);
+  m.impl("dequantize_mxfp4", &dequantize_mxfp4);
+  m.impl("gemm_mxfp4", &gemm_mxfp4);
+  m.impl("linear_mxfp4", &linear_mxfp4);
+  m.impl("moe", &moe);
+  m.impl("moe_experts", &moe_experts);
+}
+
+TORCH_LIBRARY_IMPL(blockfp8_b200, CPU, m) { impl_experts(m); }
+
 TORCH_LIBRARY_IMPL(blockfp8_b200, CUDA, m) {
+  impl_experts(m);
   m.impl("rms_norm_quant", &rms_norm_quant);
   m.impl("silu_mul_quant", &silu_mul_quant);
 }

@@ -450,4 +450,76 @@ __host__ __device__ constexpr uint32_t idesc_e4m3_f32(int m, int n) {
   return (1u << 4) | (uint32_t(n >> 3) << 17) | (uint32_t(m >> 4) << 24);
 }
 
+// ---- block-scaled MXFP4 (kind::mxf4) --------------------------------------------
+
+// Untiled copy of `bytes` (a multiple of 16; both addresses 16-byte aligned)
+// into this CTA's shared memory, completing them on the barrier.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar,
+                                          uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;" ::"r"(
+          dst),
+      "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+      : "memory");
+}
+
+// 32 rows of 16 bytes from shared memory (512 contiguous bytes) into 4 TMEM
+// columns, the same 32 lanes repeated in each warp's quarter: the scale
+// factors of a 128-row x 128-column tile.  Ordered before MMAs that the same
+// thread issues after it.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// The same from each CTA of a pair into its own TMEM.
+__device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
+  asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+
+// Matrix descriptor of such a 512-byte scale tile: no swizzle, 8-row groups
+// 128 bytes apart, descriptor version 1.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
+}
+
+// D[tmem] (+)= (A * scale_A) (B * scale_B)^T over K = 64 e2m1 values, one
+// E8M0 scale per 32 (scale_vec::2X) from TMEM.
+template <int CG = 1>
+__device__ __forceinline__ void mma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+            d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+        : "memory");
+}
+
+// Instruction descriptor of kind::mxf4: A and B E2M1 (format 1 in bits 7-9
+// and 10-11), both K-major, N >> 3 in bits 17-22, scales E8M0 (bit 23),
+// M >> 7 in bits 27-28; which half of a 4-byte scale word an MMA reads (0 or
+// 2) goes into bits 4-5 (B) and 29-30 (A).
+__host__ __device__ constexpr uint32_t idesc_mxf4(int m, int n) {
+  return (1u << 7) | (1u << 10) | (uint32_t(n >> 3) << 17) | (1u << 23) | (uint32_t(m >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t idesc_scale_half(int half) {
+  return (uint32_t(2 * half) << 4) | (uint32_t(2 * half) << 29);
+}
+
+// The shared::cluster address's float (distributed shared memory).
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+
 }  // namespace bfp8

@@ -272,6 +272,97 @@ typedef struct bfp8_silu_mul_quant_problem {
 } bfp8_silu_mul_quant_problem;
 int bfp8_launch_silu_mul_quant(const bfp8_silu_mul_quant_problem* p, void* stream);
 
+/* ---- MXFP4 (OCP microscaling, 4 bit).  No reference counterpart. ------------
+ *
+ * e2m1 codes, two to a byte (value 2j in the low nibble of byte j), and one
+ * power-of-two scale byte (E8M0) per 32 values of a row:
+ *   byte = max(floor(log2(amax)) - 2, -127) + 127, code = e2m1(x 2^-(byte - 127))
+ * to nearest even, at most 6 in magnitude; a block with an infinity or a NaN
+ * gets byte 255 (NaN).  Scales live in tiles of 128 rows x 128 columns,
+ * [ceil(R/128), ceil(K/128), 32, 16]: row r of a tile at [r % 32], its four
+ * bytes at 4 (r / 32); bytes past the matrix are zero.  K is a multiple of
+ * 32; rows of codes are 16-byte aligned. */
+
+/* x [M, K] (x_type 0: fp32, 1: bf16, 2: fp16; rows 16-byte aligned) -> q, s. */
+typedef struct bfp8_mxfp4_quant_problem {
+  const void* x;
+  int64_t ldx;
+  int x_type;
+  void* q;
+  int64_t ldq; /* bytes */
+  void* s;
+  int M, K;
+} bfp8_mxfp4_quant_problem;
+int bfp8_launch_mxfp4_quantize(const bfp8_mxfp4_quant_problem* p, void* stream);
+
+/* q, s -> the values they stand for, y [M, K] (y_type 0: fp32, 1: bf16). */
+typedef struct bfp8_mxfp4_dequant_problem {
+  const void* q;
+  int64_t ldq;
+  const void* s;
+  void* y;
+  int64_t ldy;
+  int y_type;
+  int M, K;
+} bfp8_mxfp4_dequant_problem;
+int bfp8_launch_mxfp4_dequantize(const bfp8_mxfp4_dequant_problem* p, void* stream);
+
+/* C [M, N] bf16 = A [M, K] B [N, K]^T, both MXFP4, accumulated in fp32.  N a
+ * multiple of 8.  weights_ready != 0: every kernel that wrote b or sb has
+ * finished before the kernel ahead of this one in the stream started (then
+ * they are requested while that kernel still runs). */
+typedef struct bfp8_mxfp4_gemm_problem {
+  const void* a;
+  int64_t lda; /* bytes */
+  const void* sa;
+  const void* b;
+  int64_t ldb;
+  const void* sb;
+  void* c;
+  int64_t ldc;
+  int M, N, K;
+  int weights_ready;
+} bfp8_mxfp4_gemm_problem;
+int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* p, void* stream);
+
+/* ---- A mixture-of-experts layer for a few tokens.  No reference counterpart.
+ *
+ *   y[t] = sum_j p[t, j] W2[e] (silu(W1[e] x[t]) * (W3[e] x[t])),  e = ids[t, j]
+ *
+ * Routing: logits [T, E] (ids null): the top_k largest, ties to the lower
+ * index, -inf and NaN never chosen; p is the softmax over all experts
+ * (renormalize = 0) or over the chosen ones.  Or ids [T, top_k] int32 and
+ * weights [T, top_k] fp32 (logits null); an id outside [0, E) adds nothing.
+ * w13 [E, 2 I, H] holds W1 (gate) over W3 (up); w2 [E, H, I].  format 0: block
+ * FP8 (e4m3, scales fp32 [E, ceil(rows/128), ceil(K/128)]); 1: MXFP4 (codes
+ * [E, rows, K/2], scale tiles [E, ceil(rows/128), ceil(K/128), 32, 16]).
+ * 1 <= T <= 64, H and I multiples of 32, 32 <= H <= 8192, E <= 512, top_k <=
+ * min(16, E).  Rows of x, y, w13 and w2 are 16-byte aligned. */
+typedef struct bfp8_moe_problem {
+  const void* x;
+  int64_t ldx;
+  int x_type; /* of x and y; 1: bf16, 2: fp16 */
+  const void* logits;
+  int64_t ld_logits;
+  int logits_type; /* 0: fp32, 1: bf16, 2: fp16 */
+  const int* ids;
+  const float* weights;
+  int renormalize;
+  int format;
+  const void* w13;
+  int64_t w13_expert, w13_row; /* bytes between experts, between rows */
+  const void* s13;
+  const void* w2;
+  int64_t w2_expert, w2_row;
+  const void* s2;
+  void* y;
+  int64_t ldy;
+  int T, H, I, E, top_k;
+} bfp8_moe_problem;
+/* Bytes of device workspace a launch needs (16-byte aligned, any contents). */
+int64_t bfp8_moe_workspace_bytes(const bfp8_moe_problem* p);
+int bfp8_launch_moe(const bfp8_moe_problem* p, void* workspace, void* stream);
+
 /* The message of the last failed call on this host thread ("" if none).
  * No reference counterpart (the reference throws std::runtime_error). */
 const char* bfp8_last_error(void);
