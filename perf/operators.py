@@ -243,10 +243,19 @@ def _moe(state):
     return (z * share.t().unsqueeze(2)).sum(0).to(state["x"].dtype)
 
 
+def _hold_bytes(state):
+    """MXFP4 codes come out of prepare()'s arithmetic in 64-bit integers.  A program holds its weights as the
+    bytes that the calls take: they are narrowed once, at a state's first pass, and kept in the state."""
+    for name in ("w", "w13", "w2"):
+        if name in state and state[name].dtype == torch.int64:
+            state[name] = state[name].to(torch.uint8)
+
+
 def run(state):
     if own:
         import blockfp8_b200 as bf
 
+        _hold_bytes(state)
         if state["op"] == "quant":
             return bf.dequantize_mxfp4(*bf.quantize_mxfp4(state["x"]))
         if state["op"] == "linear":
