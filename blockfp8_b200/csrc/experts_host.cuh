@@ -108,10 +108,10 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int nt, MoeLayout* out) {
   const int P = p.T * p.top_k, blocks = cdiv(k, 128), bb = p.format ? 64 : 128;
   const int row = blocks * bb;                      // bytes of a unit's row
   out->stage_row = round_up(cdiv(row, cdiv(row, 1024)), bb);
-  const int stage = 16 * (out->stage_row + 16);
+  const int stage = 16 * (out->stage_row + 16) + (p.format ? out->stage_row / bb * 256 : 0);
   const int b = blocks * 2048 * nt, ts = blocks * 8 * nt * 4, red = 2 * kMoeConsumers * nt * 512;
   const int route = round_up(moe_route_bytes(P), 16);
-  const int fixed = b + ts + red + route + 16 * 8 * 2 + 64 + 16;
+  const int fixed = b + ts + red + route + 16 * 8 * 2 + 64 + 16 + 4 * (1 + kMoeBatch);
   const int stages = std::min(16, (kMaxSmem - fixed) / stage);
   if (stages < kMoeMinStages) return false;
   const int scratch = p.E * cdiv(P, 32) * 4 + p.E * 4;
@@ -122,7 +122,7 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int nt, MoeLayout* out) {
   out->off_red = out->off_ts + uint32_t(round_up(ts, 16));
   out->off_route = out->off_red + uint32_t(red);
   out->off_bars = out->off_route + uint32_t(route);
-  out->smem = int(out->off_bars) + 8 * (2 * stages + 4) + 16;
+  out->smem = int(out->off_bars) + 8 * (2 * stages + 4) + 16 + 4 * (1 + kMoeBatch);
   return out->smem <= kMaxSmem;
 }
 

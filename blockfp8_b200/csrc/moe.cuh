@@ -43,6 +43,7 @@
 #include <type_traits>
 
 #include "mxfp4.cuh"
+#include "producers.cuh"
 #include "ptx.cuh"
 
 namespace bfp8 {
@@ -52,6 +53,7 @@ constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxExperts = 512;
 constexpr int kMoeConsumers = 8;
 constexpr int kMoeThreads = 32 * (kMoeConsumers + 2);
+constexpr int kMoeBatch = 16;  // units whose arrival DOWN counts together
 
 struct MoeParams {
   const void* x;  // [T, H] bf16 or fp16
@@ -267,6 +269,20 @@ __device__ __forceinline__ void e4m3x4_to_f16(uint32_t codes, uint32_t& lo, uint
       : "=r"(lo), "=r"(hi)
       : "r"(codes));
 }
+// The powers of two of four E8M0 bytes (exact; 255 is NaN).
+__device__ __forceinline__ void e8m0x4_to_float(uint32_t bytes, float (&f)[4]) {
+  uint32_t lo, hi;
+  asm("{\n\t.reg .b16 a, b;\n\t"
+      "mov.b32 {a, b}, %2;\n\t"
+      "cvt.rn.bf16x2.ue8m0x2 %0, a;\n\t"
+      "cvt.rn.bf16x2.ue8m0x2 %1, b;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(bytes));
+  f[0] = __uint_as_float(lo << 16);
+  f[1] = __uint_as_float(lo & 0xFFFF0000u);
+  f[2] = __uint_as_float(hi << 16);
+  f[3] = __uint_as_float(hi & 0xFFFF0000u);
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   const __half2 h = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -278,6 +294,38 @@ __device__ __forceinline__ void moe_act_scale(uint32_t amax_bits, float& to, flo
   const int f = amax_bits == 0u ? 127 : min(127 + 14 + 127 - e, 253);  // biased exponent of `to`
   to = __uint_as_float(uint32_t(f) << 23);
   back = __uint_as_float(uint32_t(254 - f) << 23);
+}
+
+// y of the row tiles in list[1 .. list[0]]: a thread takes four rows of one
+// token and adds its pairs in order (and each pair's K ranges in order).
+template <class T>
+__device__ void moe_combine(const MoeParams& p, const MoeRoute& route, const int* list, int thread, int threads) {
+  const int tasks = list[0] * p.T * 4;
+  for (int task = thread; task < tasks; task += threads) {
+    const int t = (task >> 2) % p.T, r0 = list[1 + (task >> 2) / p.T] * 16 + (task & 3) * 4;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int j = 0; j < p.top_k; ++j) {
+      const int pair = t * p.top_k + j;
+      if (route.expert[pair] < 0) continue;
+      const float* z = p.z + int64_t(pair) * p.segments * p.H + r0;
+      float4 v = __ldcg(reinterpret_cast<const float4*>(z));
+      for (int sg = 1; sg < p.segments; ++sg) {
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(z + int64_t(sg) * p.H));
+        v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+      }
+      const float w = route.weight[pair];
+      sum.x = fmaf(w, v.x, sum.x), sum.y = fmaf(w, v.y, sum.y);
+      sum.z = fmaf(w, v.z, sum.z), sum.w = fmaf(w, v.w, sum.w);
+    }
+    T* y = static_cast<T*>(p.y) + int64_t(t) * p.ldy + r0;
+    uint2 out;
+    if constexpr (std::is_same_v<T, __nv_bfloat16>)
+      out = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+    else
+      out = make_uint2(pack_f16x2(sum.x, sum.y), pack_f16x2(sum.z, sum.w));
+    *reinterpret_cast<uint2*>(y) = out;
+  }
 }
 
 template <bool GATE_, bool MX_, int NT_, class T_>
@@ -297,12 +345,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
   const uint32_t base = smem_u32(smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = p.stages, row_pitch = p.stage_row + 16;
-  const uint32_t stage_bytes = uint32_t(16 * row_pitch);
+  const uint32_t stage_bytes = uint32_t(16 * row_pitch + (MX ? p.stage_row / BB * 256 : 0));
   auto full = [&](int s) { return base + p.off_bars + 8u * uint32_t(s); };
   auto empty = [&](int s) { return base + p.off_bars + 8u * uint32_t(S + s); };
   auto red_full = [&](int b) { return base + p.off_bars + 8u * uint32_t(2 * S + b); };
   auto red_empty = [&](int b) { return base + p.off_bars + 8u * uint32_t(2 * S + 2 + b); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + p.off_bars + 8 * (2 * S + 4));
+  int* finished = reinterpret_cast<int*>(smem + p.off_bars + 8 * (2 * S + 4) + 16);  // [1 + kMoeBatch]
   const MoeRoute route = moe_route_at(smem + p.off_route, p.T * p.top_k);
 
   if (tid == 0) {
@@ -315,6 +364,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
       mbar_init(red_empty(b), 1u);
     }
     *abort_flag = 0;
+    finished[0] = 0;
     fence_barrier_init();
   }
   if constexpr (GATE) {
@@ -341,7 +391,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
 
   if (warp == kMoeConsumers) {
     // ---------------------------------------------------------------- producer
-    const uint64_t policy = policy_evict_first();
+    const uint64_t policy = policy_evict_first(), scale_policy = policy_evict_normal();
     int n = 0;
     bool ok = true;
     for (int u = u0; u < u1 && ok; ++u) {
@@ -358,9 +408,23 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
         ok = __all_sync(~0u, ok);
         if (!ok) break;
         const uint32_t len = uint32_t(min(p.stage_row, bytes - at));
-        if (lane == 0) mbar_arrive_expect_tx(full(s), 16u * len);
+        const int nb = (int(len) + BB - 1) / BB;
+        const uint32_t stage = base + uint32_t(s) * stage_bytes;
+        if (lane == 0) mbar_arrive_expect_tx(full(s), 16u * len + (MX ? uint32_t(nb) * 256u : 0u));
         __syncwarp();
-        if (lane < 16) bulk_load(base + uint32_t(s) * stage_bytes + uint32_t(lane * row_pitch), src + at, len, full(s), policy);
+        if (lane < 16) bulk_load(stage + uint32_t(lane * row_pitch), src + at, len, full(s), policy);
+        if constexpr (MX) {
+          // A block's scale words of 8 rows are 8 x 16 contiguous bytes of its
+          // tile, each with the words of the rows 32, 64 and 96 further on:
+          // a fourth of it is used here, the rest by the CTA's next units (from L2).
+          const int half = lane >> 4;  // rows 0-7 and 8-15 of the unit
+          const int r = GATE ? half * p.I + tile * 8 : tile * 16 + 8 * half;
+          const uint8_t* sc = static_cast<const uint8_t*>(p.ws) +
+                              ((int64_t(route.chunk_expert[chunk]) * p.rb + (r >> 7)) * p.kb + seg * (p.seg_len / 128) + at / BB) * 512 +
+                              (r & 31) * 16;
+          for (int i = lane & 15; i < nb; i += 16)
+            bulk_load(stage + uint32_t(16 * row_pitch + i * 256 + half * 128), sc + i * 512, 128u, full(s), scale_policy);
+        }
       }
     }
     for (int k = n > S ? n - S : 0; k < n; ++k) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMoeWaitDrain);
@@ -370,18 +434,41 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
     uint8_t* bfrag = smem + p.off_b;
     float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8 NT]
     if constexpr (!GATE) griddep_wait();                    // h
-    int n = 0, q = 0, have = -1, count = 0, experts_row = 0;
+    int n = 0, q = 0, have = -1, count = 0;
     bool ok = true;
+    // Block FP8 scales: lane l holds those of K blocks l and l + 32 of the
+    // unit's two 8-row halves, requested a unit ahead.
+    float sc[2][2], sc_next[2][2];
+    auto load_scales = [&](int u, float (&v)[2][2]) {
+      int chunk, seg, tile;
+      place(u, chunk, seg, tile);
+      const float* e = static_cast<const float*>(p.ws) + int64_t(route.chunk_expert[chunk]) * p.rb * p.kb;
+      const int kb = seg * (p.seg_len / 128);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int r = GATE ? half * p.I + tile * 8 : tile * 16 + 8 * half;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int b = kb + lane + 32 * j;
+          v[half][j] = b < p.kb ? ldg_pinned(e + int64_t(r >> 7) * p.kb + b) : 0.f;
+        }
+      }
+    };
+    if (!MX && u0 < u1) load_scales(u0, sc_next);
     for (int u = u0; u < u1; ++u) {
       int chunk, seg, tile;
       place(u, chunk, seg, tile);
+      if constexpr (!MX) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) sc[half][0] = sc_next[half][0], sc[half][1] = sc_next[half][1];
+        if (u + 1 < u1) load_scales(u + 1, sc_next);
+      }
       const int k_len = min(p.seg_len, K - seg * p.seg_len);
       const int blocks = (k_len + 127) / 128;
       if (have != chunk * p.segments + seg) {
         // ---- the chunk's activations to f16 fragments
         have = chunk * p.segments + seg;
         count = route.chunk_count[chunk];
-        experts_row = route.chunk_expert[chunk];
         named_bar_sync(1, 32 * kMoeConsumers);
         const int half = tid >> 4, l16 = tid & 15;  // 16 half-warps; a task is one token's block
         const int tasks = count * blocks;
@@ -427,8 +514,6 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
         }
         named_bar_sync(1, 32 * kMoeConsumers);
       }
-      // The unit's scales: fp32 of the two 8-row halves, or the rows' bytes.
-      const int row_a = GATE ? tile * 8 : tile * 16, row_b = GATE ? p.I + tile * 8 : tile * 16 + 8;
       float acc[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
@@ -437,19 +522,18 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
         ok = mbar_wait(full(s), uint32_t(n / S) & 1u, abort_flag, kMoeWaitFull) && ok;
         const int nb = min(stage_blocks, blocks - b0);
         for (int i = (warp - q) & (kMoeConsumers - 1); i < nb; i += kMoeConsumers) {
-          const int b = b0 + i;                       // block of this K range
-          const int kb = seg * (p.seg_len / 128) + b;  // block of the matrix
-          float sa = 0.f, sb = 0.f;
-          uint32_t ea = 0u, eb = 0u;
+          const int b = b0 + i;  // block of this K range
+          float sa = 1.f, sb = 1.f;
+          float fa4[4], fb4[4];
           if constexpr (MX) {
-            const uint8_t* sc = static_cast<const uint8_t*>(p.ws) + int64_t(experts_row) * p.rb * p.kb * 512;
-            const int ra = row_a + g, rb = row_b + g;
-            ea = *reinterpret_cast<const uint32_t*>(sc + (int64_t(ra >> 7) * p.kb + kb) * 512 + (ra & 31) * 16 + ((ra >> 5) & 3) * 4);
-            eb = *reinterpret_cast<const uint32_t*>(sc + (int64_t(rb >> 7) * p.kb + kb) * 512 + (rb & 31) * 16 + ((rb >> 5) & 3) * 4);
+            // the word of this row: 32-row quarter of its tile
+            const int ra = (GATE ? tile * 8 : tile * 16), rb = GATE ? p.I + tile * 8 : tile * 16 + 8;
+            const uint32_t at = base + uint32_t(s) * stage_bytes + uint32_t(16 * row_pitch + i * 256 + g * 16);
+            e8m0x4_to_float(ld_shared_u32(at + uint32_t((ra >> 5) & 3) * 4u), fa4);
+            e8m0x4_to_float(ld_shared_u32(at + 128u + uint32_t((rb >> 5) & 3) * 4u), fb4);
           } else {
-            const float* sc = static_cast<const float*>(p.ws) + int64_t(experts_row) * p.rb * p.kb;
-            sa = sc[int64_t(row_a >> 7) * p.kb + kb];
-            sb = GATE ? sc[int64_t(row_b >> 7) * p.kb + kb] : sa;
+            sa = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][1], b & 31);
+            sb = GATE ? __shfl_sync(~0u, b < 32 ? sc[1][0] : sc[1][1], b & 31) : sa;
           }
           // ldmatrix rows: lanes 0-7 / 8-15 the two row halves of one 16-byte
           // column, lanes 16-31 of the next
@@ -471,7 +555,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
                     uint32_t ha[4], hb[4];
                     e2m1x8_to_f16(r[2 * h2], ha);
                     e2m1x8_to_f16(r[2 * h2 + 1], hb);
-                    const float fa = e8m0_value((ea >> (8 * (pp + h2))) & 255u), fb = e8m0_value((eb >> (8 * (pp + h2))) & 255u);
+                    const float fa = fa4[pp + h2], fb = fb4[pp + h2];
 #pragma unroll
                     for (int c = 0; c < NT; ++c) {
                       if (c == 0 || c * 8 < count) {
@@ -512,11 +596,10 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
           for (int c = 0; c < NT; ++c) {
             if (c == 0 || c * 8 < count) {
               const float2 tsc = *reinterpret_cast<const float2*>(ts + b * 8 * NT + c * 8 + 2 * t4);
-              const float fa = MX ? 1.f : sa, fb = MX ? 1.f : sb;
-              acc[c][0] = fmaf(part[c][0], tsc.x * fa, acc[c][0]);
-              acc[c][1] = fmaf(part[c][1], tsc.y * fa, acc[c][1]);
-              acc[c][2] = fmaf(part[c][2], tsc.x * fb, acc[c][2]);
-              acc[c][3] = fmaf(part[c][3], tsc.y * fb, acc[c][3]);
+              acc[c][0] = fmaf(part[c][0], tsc.x * sa, acc[c][0]);
+              acc[c][1] = fmaf(part[c][1], tsc.y * sa, acc[c][1]);
+              acc[c][2] = fmaf(part[c][2], tsc.x * sb, acc[c][2]);
+              acc[c][3] = fmaf(part[c][3], tsc.y * sb, acc[c][3]);
             }
           }
         }
@@ -543,6 +626,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
       for (int64_t i = int64_t(blockIdx.x) * 32 + lane; i < int64_t(p.T) * p.H; i += int64_t(gridDim.x) * 32)
         y[i / p.H * p.ldy + i % p.H] = T(0.f);
     }
+    int flushed = u0;  // units whose arrival is counted
     for (int u = u0; u < u1; ++u) {
       int chunk, seg, tile;
       place(u, chunk, seg, tile);
@@ -577,40 +661,33 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
       __syncwarp();
       if (lane == 0) mbar_arrive(red_empty(buf));
       if constexpr (!GATE) {
-        // ---- the last unit of an output row tile adds its pairs
-        __threadfence();
-        int last = 0;
-        if (lane == 0) last = atomicAdd(p.counters + tile, 1) == chunks * p.segments - 1;
-        last = __shfl_sync(~0u, last, 0);
-        if (last) {
+        // Arrivals are counted a batch of units at a time: a fence and an
+        // atomic cost as much as streaming two to four units.
+        if (u + 1 - flushed == kMoeBatch || u + 1 == u1) {
           __threadfence();
-          const int r0 = tile * 16 + t4 * 4;  // four output rows a lane, eight tokens a pass
-          for (int t = g; t < p.T; t += 8) {
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int j = 0; j < p.top_k; ++j) {
-              const int pair = t * p.top_k + j;
-              if (route.expert[pair] < 0) continue;
-              float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-              for (int sg = 0; sg < p.segments; ++sg) {
-                const float4 a = __ldcg(reinterpret_cast<const float4*>(p.z + (int64_t(pair) * p.segments + sg) * p.H + r0));
-                v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
-              }
-              const float w = route.weight[pair];
-              sum.x = fmaf(w, v.x, sum.x), sum.y = fmaf(w, v.y, sum.y);
-              sum.z = fmaf(w, v.z, sum.z), sum.w = fmaf(w, v.w, sum.w);
-            }
-            T* y = static_cast<T*>(p.y) + int64_t(t) * p.ldy + r0;
-            if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-              reinterpret_cast<__nv_bfloat162*>(y)[0] = __floats2bfloat162_rn(sum.x, sum.y);
-              reinterpret_cast<__nv_bfloat162*>(y)[1] = __floats2bfloat162_rn(sum.z, sum.w);
-            } else {
-              reinterpret_cast<__half2*>(y)[0] = __floats2half2_rn(sum.x, sum.y);
-              reinterpret_cast<__half2*>(y)[1] = __floats2half2_rn(sum.z, sum.w);
-            }
+          __syncwarp();
+          bool last = false;
+          int tile_l = 0;
+          if (lane < u + 1 - flushed) {
+            int c_l, s_l;
+            place(flushed + lane, c_l, s_l, tile_l);
+            last = atomicAdd(p.counters + tile_l, 1) == chunks * p.segments - 1;
           }
+          __threadfence();
+          const uint32_t lasts = __ballot_sync(~0u, last);
+          if (last) finished[1 + __popc(lasts & ((1u << lane) - 1u))] = tile_l;
+          if (lane == 0) finished[0] = __popc(lasts);
+          __syncwarp();
+          flushed = u + 1;
+          if (u + 1 < u1) moe_combine<T>(p, route, finished, lane, 32);
         }
       }
     }
+  }
+  if constexpr (!GATE) {
+    __syncthreads();
+    // the last batch's row tiles, by every warp
+    if (!*abort_flag) moe_combine<T>(p, route, finished, tid, kMoeThreads);
   }
 }
 
