@@ -85,57 +85,101 @@ int launch_mx_gemm(MxGemmParams& gp, const bfp8_mxfp4_gemm_problem& p, int dev, 
 
 // ---- the expert layer ---------------------------------------------------------------
 
-struct MoeShape {
-  int nt;        // 8-token tiles of a chunk
-  int segments;  // K ranges of DOWN
-  int seg_len;
-};
-
 constexpr int kMoeMaxHidden = 8192;
 constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
 constexpr int kMoeMinStages = 3;
+constexpr int kMoeHalfSmem = 113 * 1024;
 
 int round_up(int x, int m) { return cdiv(x, m) * m; }
 
+// How one kernel's units (segments of seg_len values of K) and shared memory
+// are laid out.
 struct MoeLayout {
-  int stages, stage_row, smem;
+  int segments, seg_len, box, stages, smem;
   uint32_t off_b, off_ts, off_red, off_route, off_bars;
 };
 
-// Shared memory of one kernel whose units span k values: as many stages as
-// fit beside the activations.
-bool moe_layout(const bfp8_moe_problem& p, int k, int nt, MoeLayout* out) {
-  const int P = p.T * p.top_k, blocks = cdiv(k, 128), bb = p.format ? 64 : 128;
-  const int row = blocks * bb;                      // bytes of a unit's row
-  out->stage_row = round_up(cdiv(row, cdiv(row, 1024)), bb);
-  const int stage = 16 * (out->stage_row + 16) + (p.format ? out->stage_row / bb * 256 : 0);
-  const int b = blocks * 2048 * nt, ts = blocks * 8 * nt * 4, red = 2 * kMoeConsumers * nt * 512;
-  const int route = round_up(moe_route_bytes(P), 16);
-  const int fixed = b + ts + red + route + 16 * 8 * 2 + 64 + 16 + 4 * (1 + kMoeBatch);
-  const int stages = std::min(16, (kMaxSmem - fixed) / stage);
-  if (stages < kMoeMinStages) return false;
-  const int scratch = p.E * cdiv(P, 32) * 4 + p.E * 4;
-  if (stages * stage < scratch) return false;
+// K of `k` values in `segments` ranges; as many stages as fit beside a range's
+// activations, in half an SM's shared memory where four do -- DOWN then starts
+// beside GATE and requests its weights while GATE runs -- else in all of it.
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int nt, MoeLayout* out) {
+  const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
+  const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, 8);
+  out->box = cdiv(columns, unit_stages);
+  out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
+  out->segments = cdiv(k, out->seg_len);
+  const int blocks = cdiv(std::min(k, out->seg_len), 128);
+  const int stage = round_up(out->box * (2048 + (p.format ? 512 : 0)), 1024);
+  const int b = blocks * 256 * std::min(p.T, 8 * nt), ts = round_up(blocks * 8 * nt * 4, 16);
+  const int red = 2 * kMoeConsumers * nt * 512, route = round_up(moe_route_bytes(P), 16);
+  const int scratch = P > 32 ? p.E * (cdiv(P, 32) + 1) * 4 : 0;
+  auto end_of = [&](int stages) { return 8 * (2 * stages + 4) + 16; };
+  const int fixed = 1024 + b + ts + red + route + end_of(16);
+  int stages = std::min(16, (kMoeHalfSmem - fixed) / stage);
+  if (stages < 4 || stages * stage < scratch) stages = std::min(16, (kMaxSmem - fixed) / stage);
+  if (stages < kMoeMinStages || stages * stage < scratch) return false;
   out->stages = stages;
-  out->off_b = uint32_t(round_up(stages * stage, 128));
+  out->off_b = uint32_t(stages * stage);
   out->off_ts = out->off_b + uint32_t(b);
-  out->off_red = out->off_ts + uint32_t(round_up(ts, 16));
+  out->off_red = out->off_ts + uint32_t(ts);
   out->off_route = out->off_red + uint32_t(red);
   out->off_bars = out->off_route + uint32_t(route);
-  out->smem = int(out->off_bars) + 8 * (2 * stages + 4) + 16 + 4 * (1 + kMoeBatch);
-  return out->smem <= kMaxSmem;
+  out->smem = 1024 + int(out->off_bars) + end_of(stages);
+  return true;
 }
+
+struct MoeShape {
+  int nt;  // 8-token tiles of a chunk
+  MoeLayout gate, down;
+};
 
 // Tokens of a chunk: 16 where the batch can fill them and the activations of
 // both kernels leave room for the ring, else 8.
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
-  s->segments = cdiv(p.I, kMoeSegment);
-  s->seg_len = round_up(cdiv(p.I, s->segments), 128);
-  s->segments = cdiv(p.I, s->seg_len);
-  MoeLayout lay;
   for (s->nt = p.T > 8 ? 2 : 1; s->nt >= 1; --s->nt)
-    if (moe_layout(p, p.H, s->nt, &lay) && moe_layout(p, std::min(p.I, s->seg_len), s->nt, &lay)) return true;
+    if (moe_layout(p, p.H, 1, s->nt, &s->gate) && moe_layout(p, p.I, cdiv(p.I, kMoeSegment), s->nt, &s->down)) return true;
   return false;
+}
+
+// Tensor maps of one stack of expert weights [E, rows, k] and its scales.
+int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int64_t w_expert, int64_t w_row,
+             const void* scales, int E, int rows, int k) {
+  const uint64_t bytes = uint64_t(format ? k / 2 : k), full = bytes / 128;
+  mp.columns = int(full);
+  if (E == 1) w_expert = w_row * rows;  // one expert's stride says nothing
+  auto fn = encode_fn();
+  if (!fn) return fail(BFP8_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  auto encode = [&](CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
+                    const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
+    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, ones,
+                    CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(BFP8_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
+    return int(BFP8_OK);
+  };
+  if (full > 0) {  // [128 bytes][rows][columns][experts]
+    const cuuint64_t dims[4] = {128, cuuint64_t(rows), full, cuuint64_t(E)};
+    const cuuint64_t strides[3] = {cuuint64_t(w_row), 128, cuuint64_t(w_expert)};
+    const cuuint32_t box[4] = {128, 8, cuuint32_t(lay.box), 1};
+    if (int r = encode(&mp.map_w, w, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return r;
+  }
+  if (bytes % 128) {
+    const cuuint64_t dims[3] = {bytes, cuuint64_t(rows), cuuint64_t(E)};
+    const cuuint64_t strides[2] = {cuuint64_t(w_row), cuuint64_t(w_expert)};
+    const cuuint32_t box[3] = {128, 8, 1};
+    if (int r = encode(&mp.map_tail, w, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return r;
+  }
+  mp.rb = cdiv(rows, 128);
+  mp.kb = cdiv(k, 128);
+  mp.ws = scales;
+  if (format) {  // [512 bytes of a tile][K blocks][row tiles][experts]
+    const cuuint64_t dims[4] = {512, cuuint64_t(mp.kb), cuuint64_t(mp.rb), cuuint64_t(E)};
+    const cuuint64_t strides[3] = {512, cuuint64_t(mp.kb) * 512, cuuint64_t(mp.rb) * mp.kb * 512};
+    const cuuint32_t box[4] = {128, cuuint32_t(2 * lay.box), 1, 1};
+    if (int r = encode(&mp.map_s, scales, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return r;
+  }
+  return BFP8_OK;
 }
 
 int check_moe(const bfp8_moe_problem& p) {
@@ -167,13 +211,16 @@ template <class Cfg>
 int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   if (int r = allow_smem(reinterpret_cast<const void*>(&moe_kernel<Cfg>), kMaxSmem, dev, done)) return r;
+  mp.segments = lay.segments;
+  mp.seg_len = lay.seg_len;
   mp.stages = lay.stages;
-  mp.stage_row = lay.stage_row;
+  mp.box = lay.box;
   mp.off_b = lay.off_b;
   mp.off_ts = lay.off_ts;
   mp.off_red = lay.off_red;
   mp.off_route = lay.off_route;
   mp.off_bars = lay.off_bars;
+  mp.cols = std::min(mp.T, 8 * Cfg::NT);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(num_sms));
   cfg.blockDim = dim3(kMoeThreads);
@@ -288,7 +335,7 @@ int64_t bfp8_moe_workspace_bytes(const bfp8_moe_problem* pp) {
   MoeShape s;
   if (!moe_shape(p, &s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
   const int64_t pairs = int64_t(p.T) * p.top_k;
-  return align256(pairs * p.I * 4) + align256(pairs * s.segments * p.H * 4) + align256(int64_t(p.H) / 16 * 4);
+  return align256(pairs * p.I * 4) + align256(pairs * s.down.segments * p.H * 4) + align256(pairs * 8);
 }
 
 int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
@@ -315,36 +362,29 @@ int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
   mp.renormalize = p.renormalize;
   mp.h = reinterpret_cast<float*>(ws);
   mp.z = reinterpret_cast<float*>(ws + align256(pairs * p.I * 4));
-  mp.counters = reinterpret_cast<int*>(ws + align256(pairs * p.I * 4) + align256(pairs * s.segments * p.H * 4));
-  mp.y = p.y;
-  mp.ldy = p.ldy;
+  mp.routed = reinterpret_cast<float2*>(ws + align256(pairs * p.I * 4) + align256(pairs * s.down.segments * p.H * 4));
   mp.T = p.T;
   mp.H = p.H;
   mp.I = p.I;
   mp.E = p.E;
   mp.top_k = p.top_k;
-  MoeLayout lay;
-  moe_layout(p, p.H, s.nt, &lay);
-  mp.w = static_cast<const uint8_t*>(p.w13);
-  mp.w_expert = p.w13_expert;
-  mp.w_row = p.w13_row;
-  mp.ws = p.s13;
-  mp.rb = cdiv(2 * p.I, 128);
-  mp.kb = cdiv(p.H, 128);
-  mp.segments = 1;
-  mp.seg_len = round_up(p.H, 128);
-  if (int r = launch_moe_any<true>(mp, lay, p.format, s.nt, p.x_type, dev, num_sms, static_cast<cudaStream_t>(stream)))
-    return r;
-  moe_layout(p, std::min(p.I, s.seg_len), s.nt, &lay);
-  mp.w = static_cast<const uint8_t*>(p.w2);
-  mp.w_expert = p.w2_expert;
-  mp.w_row = p.w2_row;
-  mp.ws = p.s2;
-  mp.rb = cdiv(p.H, 128);
-  mp.kb = cdiv(p.I, 128);
-  mp.segments = s.segments;
-  mp.seg_len = s.seg_len;
-  return launch_moe_any<false>(mp, lay, p.format, s.nt, p.x_type, dev, num_sms, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (int r = moe_maps(mp, s.gate, p.format, p.w13, p.w13_expert, p.w13_row, p.s13, p.E, 2 * p.I, p.H)) return r;
+  if (int r = launch_moe_any<true>(mp, s.gate, p.format, s.nt, p.x_type, dev, num_sms, st)) return r;
+  if (int r = moe_maps(mp, s.down, p.format, p.w2, p.w2_expert, p.w2_row, p.s2, p.E, p.H, p.I)) return r;
+  if (int r = launch_moe_any<false>(mp, s.down, p.format, s.nt, p.x_type, dev, num_sms, st)) return r;
+  const MoeSumParams sp{mp.z, mp.routed, p.y, p.ldy, p.T, p.H, p.top_k, s.down.segments};
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(cdiv(p.T * (p.H / 4), kMoeSumThreads)));
+  cfg.blockDim = dim3(kMoeSumThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  set_pdl(cfg, attr);
+  cudaError_t e = p.x_type == 1 ? cudaLaunchKernelEx(&cfg, moe_sum_kernel<__nv_bfloat16>, sp)
+                                : cudaLaunchKernelEx(&cfg, moe_sum_kernel<__half>, sp);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "expert layer sum launch");
+  return BFP8_OK;
 }
 
 }  // extern "C"

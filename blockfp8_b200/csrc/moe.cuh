@@ -1,8 +1,10 @@
-// A mixture-of-experts layer for a few tokens, in two kernels:
+// A mixture-of-experts layer for a few tokens, in two kernels that stream the
+// weights and a small sum:
 //
 //   moe_kernel<GATE>  ids, p = router(logits)            (every CTA, from the logits)
 //                     h[t, j] = silu(W1[e] x[t]) * (W3[e] x[t]),  e = ids[t, j]
-//   moe_kernel<DOWN>  z[t, j] = W2[e] h[t, j],  y[t] = sum_j p[t, j] z[t, j]
+//   moe_kernel<DOWN>  z[t, j] = W2[e] h[t, j]
+//   moe_sum_kernel    y[t] = sum_j p[t, j] z[t, j]
 //
 // Expert weights are block FP8 (e4m3, one fp32 scale per 128 x 128) or MXFP4
 // (e2m1, one power-of-two scale per 32); activations are not quantized.  At
@@ -15,11 +17,14 @@
 //   chunk over a whole K range, and CTA b of G takes units [U b / G, U (b+1) / G).
 //   16 rows keep the last wave short (one token, 8 experts of I = 768: 768
 //   units over 148 CTAs) and need no sums across CTAs.
-// - A ring of shared-memory stages, 16 rows x up to 1 KB each, filled by one
-//   warp with one bulk copy per row; it runs across units, so the memory
-//   system sees one stream per SM.  Rows are padded by 16 bytes, which makes
-//   ldmatrix conflict-free.
-// - Eight consumer warps take the 128-wide K blocks of a stage in turn:
+// - A ring of shared-memory stages, 16 rows x up to 1 KB each; it runs across
+//   units, so the memory system sees one stream per SM.  Each half of a stage
+//   (8 rows) is one 4-D TMA box [128 bytes, 8 rows, up to 8 columns of 128
+//   bytes, 1 expert] in the 128-byte swizzle, which ldmatrix reads without
+//   conflicts.  (One bulk copy per row took the issuing warp about 60 clocks
+//   each, 1,000 a stage: more than the 700 that HBM takes to deliver it.)
+// - Eight consumer warps in two groups take stages in turn, and the 128-wide K
+//   blocks of a stage in turn inside a group:
 //   ldmatrix, codes to f16 (exact: cvt, 128 codes per clock and SM), mma.sync
 //   m16n8k16 with fp32 accumulation, then the block's scales in fp32.  The
 //   legacy MMA is no bound here (one 8-token MMA per 256 weights is 0.09 of
@@ -29,9 +34,11 @@
 //   one power-of-two scale per token and 128 values, which puts the largest
 //   at 2^14: bf16 values are exact down to 2^-28 of it, and h (fp32) keeps 11
 //   bits, 8 times finer than a bf16 h would.
-// - A last warp finishes units: it adds the eight warps' sums in warp order
-//   and, DOWN, the last unit to arrive at an output row tile (a counter)
-//   adds its pairs in j order.  No result depends on the order of arrival.
+// - A last warp finishes units: it adds the eight warps' sums in warp order.
+//   z goes to memory and a small third kernel adds each token's pairs in j
+//   order.  (Counting arrivals and letting the last unit of an output row tile
+//   add them makes the slowest CTA do nearly all of it: 2.4 times the median
+//   CTA's time at 64 tokens.)  No result depends on the order of arrival.
 //
 // Warps: 0-7 consumers, 8 producer, 9 finisher.
 #pragma once
@@ -51,9 +58,9 @@ namespace bfp8 {
 constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxExperts = 512;
-constexpr int kMoeConsumers = 8;
+constexpr int kMoeConsumers = 8;  // warps, in groups that take stages in turn
+constexpr int kMoeGroups = 2;
 constexpr int kMoeThreads = 32 * (kMoeConsumers + 2);
-constexpr int kMoeBatch = 16;  // units whose arrival DOWN counts together
 
 struct MoeParams {
   const void* x;  // [T, H] bf16 or fp16
@@ -65,19 +72,29 @@ struct MoeParams {
   const int* ids;
   const float* weights;
   int renormalize;
-  const uint8_t* w;          // this kernel's weights
-  int64_t w_expert, w_row;   // bytes
-  const void* ws;            // their scales: fp32 [E, rb, kb], or E8M0 tiles [E, rb, kb, 32, 16]
+  // This kernel's weights, rows of `columns` full 128-byte columns (map_w: 8
+  // rows x box columns) and perhaps one shorter (map_tail: 8 rows x 128 bytes).
+  CUtensorMap map_w, map_tail;
+  int columns;
+  CUtensorMap map_s;  // MXFP4: scale tiles, [128 bytes = 8 rows] x 2 box K blocks
+  const void* ws;     // block FP8: scales fp32 [E, rb, kb]
   int rb, kb;
   float* h;       // [T top_k, I]
   float* z;       // [T top_k, segments, H]
-  int* counters;  // [H / 16], zeroed by GATE
-  void* y;        // [T, H]
-  int64_t ldy;
+  float2* routed;  // [T top_k] (weight, expert or -1), written by GATE
   int T, H, I, E, top_k;
-  int segments, seg_len;  // K ranges of DOWN (multiples of 128)
-  int stages, stage_row;  // ring: stages, bytes of a row per stage
+  int segments, seg_len;  // K ranges of DOWN
+  int stages, box;        // ring: stages, 128-byte columns of a stage
+  int cols;               // token columns held: min(T, 8 NT)
   uint32_t off_b, off_ts, off_red, off_route, off_bars;  // shared memory
+};
+
+struct MoeSumParams {
+  const float* z;
+  const float2* routed;
+  void* y;
+  int64_t ldy;
+  int T, H, top_k, segments;
 };
 
 enum MoeWaitSite : uint32_t {
@@ -121,66 +138,74 @@ __device__ __forceinline__ float moe_key_value(uint32_t k) {
   return __uint_as_float((k & 0x80000000u) ? (k & 0x7FFFFFFFu) : ~k);
 }
 
+// The top_k of one token by one warp: E <= 32 NE logits.
+template <int NE>
+__device__ __forceinline__ void moe_top_k(const MoeParams& p, const MoeRoute& r, int t, int lane) {
+  uint32_t key[NE];
+#pragma unroll
+  for (int i = 0; i < NE; ++i) {
+    key[i] = 0u;
+    const int e = i * 32 + lane;
+    if (e < p.E) {
+      const int64_t at = int64_t(t) * p.ld_logits + e;
+      float v;
+      if (p.logits_type == 0) v = static_cast<const float*>(p.logits)[at];
+      else if (p.logits_type == 1) v = __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]);
+      else v = __half2float(static_cast<const __half*>(p.logits)[at]);
+      key[i] = moe_key(v);
+    }
+  }
+  float all = 0.f, top = 0.f, mine = 0.f;  // lane j keeps exp(l_j - l_0) of the j-th choice
+  int id = -1, my_id = -1;
+  for (int j = 0; j < p.top_k; ++j) {
+    uint32_t best = 0u, at = ~0u;
+#pragma unroll
+    for (int i = NE - 1; i >= 0; --i)  // the lane's largest, the lowest index of equals
+      if (key[i] >= best) best = key[i], at = uint32_t(i * 32 + lane);
+    const uint32_t most = __reduce_max_sync(~0u, best);
+    if (most == 0u) break;  // nothing left to choose
+    id = int(__reduce_min_sync(~0u, best == most ? at : ~0u));
+    const float v = moe_key_value(most);
+    if (j == 0) {
+      top = v;
+      if (!p.renormalize) {
+#pragma unroll
+        for (int i = 0; i < NE; ++i)
+          if (key[i]) all += expf(moe_key_value(key[i]) - top);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+      }
+    }
+    if (lane == j) mine = v, my_id = id;
+#pragma unroll
+    for (int i = 0; i < NE; ++i)
+      if (id == i * 32 + lane) key[i] = 0u;
+  }
+  mine = my_id >= 0 ? expf(mine - top) : 0.f;
+  if (p.renormalize) {
+    all = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
+  }
+  if (lane < p.top_k) {
+    r.expert[t * p.top_k + lane] = short(my_id);
+    r.weight[t * p.top_k + lane] = my_id >= 0 ? mine / all : 0.f;
+  }
+}
+
 // The router and the chunk tables, by all threads of the CTA.  scratch: room
-// for E * ceil(P / 32) words and E ints.
-__device__ void moe_route(const MoeParams& p, const MoeRoute& r, uint32_t* scratch, int chunk_cap) {
+// for E (ceil(P / 32) + 1) words.
+__device__ void moe_route(const MoeParams& p, const MoeRoute& r, uint32_t* scratch, int cap) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int P = p.T * p.top_k, words = (P + 31) / 32;
-  uint32_t* masks = scratch;                               // [E][words]
-  int* offsets = reinterpret_cast<int*>(scratch + p.E * words);  // [E]: (first pair << 16) | first chunk
-  for (int i = tid; i < p.E * words; i += kMoeThreads) masks[i] = 0u;
+  uint32_t* masks = scratch;                                     // [E][words] pairs of each expert
+  int* offsets = reinterpret_cast<int*>(scratch + p.E * words);  // [E]
+  if (P > 32)
+    for (int i = tid; i < p.E * words; i += kMoeThreads) masks[i] = 0u;
   if (p.logits) {
     for (int t = warp; t < p.T; t += kMoeThreads / 32) {
-      uint32_t key[kMoeMaxExperts / 32];
-#pragma unroll
-      for (int i = 0; i < kMoeMaxExperts / 32; ++i) {
-        key[i] = 0u;
-        const int e = i * 32 + lane;
-        if (e < p.E) {
-          const int64_t at = int64_t(t) * p.ld_logits + e;
-          float v;
-          if (p.logits_type == 0) v = static_cast<const float*>(p.logits)[at];
-          else if (p.logits_type == 1) v = __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]);
-          else v = __half2float(static_cast<const __half*>(p.logits)[at]);
-          key[i] = moe_key(v);
-        }
-      }
-      float all = 0.f, top = 0.f, chosen = 0.f;
-      float mine = 0.f;  // lane j keeps exp(l_j - l_0) of the j-th choice
-      for (int j = 0; j < p.top_k; ++j) {
-        uint32_t best = 0u;
-#pragma unroll
-        for (int i = 0; i < kMoeMaxExperts / 32; ++i) best = max(best, key[i]);
-        best = __reduce_max_sync(~0u, best);
-        int id = -1;
-        float ex = 0.f;
-        if (best) {
-          uint32_t at = ~0u;
-#pragma unroll
-          for (int i = kMoeMaxExperts / 32 - 1; i >= 0; --i)
-            if (key[i] == best) at = uint32_t(i * 32 + lane);
-          id = int(__reduce_min_sync(~0u, at));
-          const float v = moe_key_value(best);
-          if (j == 0) {
-            top = v;
-            if (!p.renormalize) {
-#pragma unroll
-              for (int i = 0; i < kMoeMaxExperts / 32; ++i)
-                if (key[i]) all += expf(moe_key_value(key[i]) - top);
-#pragma unroll
-              for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(~0u, all, o);
-            }
-          }
-          ex = expf(v - top);
-          chosen += ex;
-#pragma unroll
-          for (int i = 0; i < kMoeMaxExperts / 32; ++i)
-            if (id == i * 32 + lane) key[i] = 0u;
-        }
-        if (lane == 0) r.expert[t * p.top_k + j] = short(id);
-        if (lane == j) mine = ex;
-      }
-      if (lane < p.top_k) r.weight[t * p.top_k + lane] = mine / (p.renormalize ? chosen : all);
+      if (p.E <= 128) moe_top_k<4>(p, r, t, lane);
+      else moe_top_k<kMoeMaxExperts / 32>(p, r, t, lane);
     }
   } else {
     for (int i = tid; i < P; i += kMoeThreads) {
@@ -190,59 +215,77 @@ __device__ void moe_route(const MoeParams& p, const MoeRoute& r, uint32_t* scrat
     }
   }
   __syncthreads();
-  for (int i = tid; i < P; i += kMoeThreads) {
-    const int e = r.expert[i];
-    if (e >= 0) atomicOr(masks + e * words + i / 32, 1u << (i & 31));
-  }
-  __syncthreads();
-  if (warp == 0) {  // first pair and first chunk of every expert
-    const int per = (p.E + 31) / 32;
-    int pairs = 0, chunks = 0;
-    for (int k = 0; k < per; ++k) {
-      const int e = lane * per + k;
-      if (e >= p.E) break;
-      int n = 0;
-      for (int w = 0; w < words; ++w) n += __popc(masks[e * words + w]);
-      pairs += n;
-      chunks += (n + chunk_cap - 1) / chunk_cap;
-    }
-    int pi = pairs, ci = chunks;
+  if (P <= 32) {
+    // One warp, a pair a lane; an expert's chunks stand where its first pair does.
+    if (warp == 0) {
+      const int e = lane < P ? r.expert[lane] : -1;
+      const uint32_t same = __match_any_sync(~0u, e);
+      const int n = e >= 0 ? __popc(same) : 0, at = __popc(same & ((1u << lane) - 1u));
+      const bool first = n > 0 && at == 0;
+      int pairs = first ? n : 0, chunks = first ? (n + cap - 1) / cap : 0;
+      const int own_pairs = pairs, own_chunks = chunks;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(~0u, pi, o), b = __shfl_up_sync(~0u, ci, o);
-      if (lane >= o) pi += a, ci += b;
-    }
-    if (lane == 31) r.totals[0] = ci;
-    pi -= pairs;
-    ci -= chunks;
-    for (int k = 0; k < per; ++k) {
-      const int e = lane * per + k;
-      if (e >= p.E) break;
-      int n = 0;
-      for (int w = 0; w < words; ++w) n += __popc(masks[e * words + w]);
-      offsets[e] = (pi << 16) | ci;
-      pi += n;
-      ci += (n + chunk_cap - 1) / chunk_cap;
-    }
-  }
-  __syncthreads();
-  for (int e = tid; e < p.E; e += kMoeThreads) {
-    const int first = offsets[e] >> 16, chunk = offsets[e] & 0xFFFF;
-    int n = 0;
-    for (int w = 0; w < words; ++w) {
-      uint32_t m = masks[e * words + w];
-      while (m) {
-        r.list[first + n++] = short(w * 32 + __ffs(m) - 1);
-        m &= m - 1;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(~0u, pairs, o), y = __shfl_up_sync(~0u, chunks, o);
+        if (lane >= o) pairs += x, chunks += y;
+      }
+      if (lane == 31) r.totals[0] = chunks;
+      const int pair0 = __shfl_sync(~0u, pairs - own_pairs, __ffs(same) - 1);
+      if (n > 0) r.list[pair0 + at] = short(lane);
+      for (int c = 0; c < own_chunks; ++c) {
+        const int k = chunks - own_chunks + c;
+        r.chunk_expert[k] = short(e);
+        r.chunk_first[k] = short(pair0 + c * cap);
+        r.chunk_count[k] = short(min(cap, n - c * cap));
       }
     }
-    for (int c = 0; c * chunk_cap < n; ++c) {
-      r.chunk_expert[chunk + c] = short(e);
-      r.chunk_first[chunk + c] = short(first + c * chunk_cap);
-      r.chunk_count[chunk + c] = short(min(chunk_cap, n - c * chunk_cap));
+  } else {
+    for (int i = tid; i < P; i += kMoeThreads) {
+      const int e = r.expert[i];
+      if (e >= 0) atomicOr(masks + e * words + i / 32, 1u << (i & 31));
     }
+    __syncthreads();
+    for (int e = tid; e < p.E; e += kMoeThreads) {
+      int n = 0;
+      for (int w = 0; w < words; ++w) n += __popc(masks[e * words + w]);
+      offsets[e] = n;
+    }
+    __syncthreads();
+    if (warp == 0) {  // first pair and first chunk of every expert
+      int pairs = 0, chunks = 0;
+      for (int e0 = 0; e0 < p.E; e0 += 32) {
+        const int e = e0 + lane, n = e < p.E ? offsets[e] : 0;
+        int pi = n, ci = (n + cap - 1) / cap;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(~0u, pi, o), y = __shfl_up_sync(~0u, ci, o);
+          if (lane >= o) pi += x, ci += y;
+        }
+        if (e < p.E) offsets[e] = ((pairs + pi - n) << 16) | (chunks + ci - (n + cap - 1) / cap);
+        pairs += __shfl_sync(~0u, pi, 31);
+        chunks += __shfl_sync(~0u, ci, 31);
+      }
+      if (lane == 0) r.totals[0] = chunks;
+    }
+    __syncthreads();
+    for (int e = tid; e < p.E; e += kMoeThreads) {
+      const int first = offsets[e] >> 16, chunk = offsets[e] & 0xFFFF;
+      int n = 0;
+      for (int w = 0; w < words; ++w) {
+        uint32_t m = masks[e * words + w];
+        while (m) {
+          r.list[first + n++] = short(w * 32 + __ffs(m) - 1);
+          m &= m - 1;
+        }
+      }
+      for (int c = 0; c * cap < n; ++c) {
+        r.chunk_expert[chunk + c] = short(e);
+        r.chunk_first[chunk + c] = short(first + c * cap);
+        r.chunk_count[chunk + c] = short(min(cap, n - c * cap));
+      }
+    }
+    fence_proxy_async_smem();  // the ring's copies overwrite the scratch next
   }
-  fence_proxy_async_smem();  // the ring's copies overwrite the scratch next
   __syncthreads();
 }
 
@@ -296,36 +339,37 @@ __device__ __forceinline__ void moe_act_scale(uint32_t amax_bits, float& to, flo
   back = __uint_as_float(uint32_t(254 - f) << 23);
 }
 
-// y of the row tiles in list[1 .. list[0]]: a thread takes four rows of one
-// token and adds its pairs in order (and each pair's K ranges in order).
+// y[t] = sum_j p[t, j] z[t, j]: a thread takes four columns of one token and
+// adds its pairs in order (and each pair's K ranges in order).
+constexpr int kMoeSumThreads = 128;
 template <class T>
-__device__ void moe_combine(const MoeParams& p, const MoeRoute& route, const int* list, int thread, int threads) {
-  const int tasks = list[0] * p.T * 4;
-  for (int task = thread; task < tasks; task += threads) {
-    const int t = (task >> 2) % p.T, r0 = list[1 + (task >> 2) / p.T] * 16 + (task & 3) * 4;
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+__global__ void __launch_bounds__(kMoeSumThreads) moe_sum_kernel(const MoeSumParams p) {
+  griddep_wait();
+  griddep_launch_dependents();
+  const int task = blockIdx.x * kMoeSumThreads + threadIdx.x;
+  const int t = task / (p.H / 4), col = task % (p.H / 4) * 4;
+  if (t >= p.T) return;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-    for (int j = 0; j < p.top_k; ++j) {
-      const int pair = t * p.top_k + j;
-      if (route.expert[pair] < 0) continue;
-      const float* z = p.z + int64_t(pair) * p.segments * p.H + r0;
-      float4 v = __ldcg(reinterpret_cast<const float4*>(z));
-      for (int sg = 1; sg < p.segments; ++sg) {
-        const float4 a = __ldcg(reinterpret_cast<const float4*>(z + int64_t(sg) * p.H));
-        v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
-      }
-      const float w = route.weight[pair];
-      sum.x = fmaf(w, v.x, sum.x), sum.y = fmaf(w, v.y, sum.y);
-      sum.z = fmaf(w, v.z, sum.z), sum.w = fmaf(w, v.w, sum.w);
+  for (int j = 0; j < p.top_k; ++j) {
+    const int pair = t * p.top_k + j;
+    const float2 r = p.routed[pair];
+    if (__float_as_int(r.y) < 0) continue;
+    const float* z = p.z + int64_t(pair) * p.segments * p.H + col;
+    float4 v = __ldcg(reinterpret_cast<const float4*>(z));
+    for (int sg = 1; sg < p.segments; ++sg) {
+      const float4 a = __ldcg(reinterpret_cast<const float4*>(z + int64_t(sg) * p.H));
+      v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
     }
-    T* y = static_cast<T*>(p.y) + int64_t(t) * p.ldy + r0;
-    uint2 out;
-    if constexpr (std::is_same_v<T, __nv_bfloat16>)
-      out = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
-    else
-      out = make_uint2(pack_f16x2(sum.x, sum.y), pack_f16x2(sum.z, sum.w));
-    *reinterpret_cast<uint2*>(y) = out;
+    sum.x = fmaf(r.x, v.x, sum.x), sum.y = fmaf(r.x, v.y, sum.y);
+    sum.z = fmaf(r.x, v.z, sum.z), sum.w = fmaf(r.x, v.w, sum.w);
   }
+  uint2 out;
+  if constexpr (std::is_same_v<T, __nv_bfloat16>)
+    out = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+  else
+    out = make_uint2(pack_f16x2(sum.x, sum.y), pack_f16x2(sum.z, sum.w));
+  *reinterpret_cast<uint2*>(static_cast<T*>(p.y) + int64_t(t) * p.ldy + col) = out;
 }
 
 template <bool GATE_, bool MX_, int NT_, class T_>
@@ -336,132 +380,235 @@ struct MoeCfg {
   static constexpr int BLOCK_BYTES = MX ? 64 : 128;  // 128 values of K of one row
 };
 
+// acc += one 128-wide K block of 16 weight rows times the chunk's tokens (C
+// tiles of 8).  a_row, chunk0: this lane's ldmatrix row and first 16-byte chunk
+// in it; b_addr: its piece of the tokens' fragments per tile, piece bytes apart
+// per 32 values of K.
+// FULL: all four 32-wide steps, so that every load can go out first; else
+// `steps` of them.
+template <class Cfg, int C, bool FULL>
+__device__ __forceinline__ void moe_block(float (&acc)[Cfg::NT][4], uint32_t a_row, uint32_t chunk0,
+                                          const uint32_t (&b_addr)[Cfg::NT], uint32_t piece, int steps, const float (&fa)[4], const float (&fb)[4],
+                                          const float* ts) {
+  // the 128-byte swizzle: chunk XOR row inside 8 rows
+  auto chunk_at = [&](uint32_t c) { return a_row + (((chunk0 + c) ^ (threadIdx.x & 7u)) << 4); };
+  float part[C][2][4];
+#pragma unroll
+  for (int c = 0; c < C; ++c)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) part[c][h][0] = part[c][h][1] = part[c][h][2] = part[c][h][3] = 0.f;
+  if constexpr (Cfg::MX) {
+    uint32_t r[4][2];  // [step][8-row half]: eight codes
+#pragma unroll
+    for (int s = 0; s < 4; s += 2)
+      if (FULL || s < steps) {
+        uint32_t v[4];
+        ldmatrix_x4(chunk_at(uint32_t(s)), v);
+        r[s][0] = v[0], r[s][1] = v[1], r[s + 1][0] = v[2], r[s + 1][1] = v[3];
+      }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (FULL || s < steps) {
+        uint32_t ha[4], hb[4];
+        e2m1x8_to_f16(r[s][0], ha);
+        e2m1x8_to_f16(r[s][1], hb);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const uint4 b = ld_shared_v4(b_addr[c] + uint32_t(s) * piece);
+          float d[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16(d, ha[0], hb[0], ha[1], hb[1], b.x, b.y);
+          mma_f16(d, ha[2], hb[2], ha[3], hb[3], b.z, b.w);
+          float(&q)[4] = part[c][s & 1];
+          q[0] = fmaf(d[0], fa[s], q[0]);
+          q[1] = fmaf(d[1], fa[s], q[1]);
+          q[2] = fmaf(d[2], fb[s], q[2]);
+          q[3] = fmaf(d[3], fb[s], q[3]);
+        }
+      }
+  } else {
+    uint32_t r[4][4];
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (FULL || s < steps) ldmatrix_x4(chunk_at(uint32_t(2 * s)), r[s]);
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+      if (FULL || s < steps) {
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e4m3x4_to_f16(r[s][k], lo[k], hi[k]);
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          const uint4 b = ld_shared_v4(b_addr[c] + uint32_t(s) * piece);
+          mma_f16(part[c][0], lo[0], lo[1], hi[0], hi[1], b.x, b.y);
+          mma_f16(part[c][1], lo[2], lo[3], hi[2], hi[3], b.z, b.w);
+        }
+      }
+  }
+  const float sa = Cfg::MX ? 1.f : fa[0], sb = Cfg::MX ? 1.f : fb[0];
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+    const float2 t = *reinterpret_cast<const float2*>(ts + c * 8);
+    acc[c][0] = fmaf(part[c][0][0] + part[c][1][0], t.x * sa, acc[c][0]);
+    acc[c][1] = fmaf(part[c][0][1] + part[c][1][1], t.y * sa, acc[c][1]);
+    acc[c][2] = fmaf(part[c][0][2] + part[c][1][2], t.x * sb, acc[c][2]);
+    acc[c][3] = fmaf(part[c][0][3] + part[c][1][3], t.y * sb, acc[c][3]);
+  }
+}
+
 template <class Cfg>
-__global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_constant__ MoeParams p) {
+__global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(const __grid_constant__ MoeParams p) {
   constexpr bool GATE = Cfg::GATE, MX = Cfg::MX;
   constexpr int NT = Cfg::NT, BB = Cfg::BLOCK_BYTES;
   using T = typename Cfg::T;
-  extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t base = smem_u32(smem);
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int S = p.stages, row_pitch = p.stage_row + 16;
-  const uint32_t stage_bytes = uint32_t(16 * row_pitch + (MX ? p.stage_row / BB * 256 : 0));
+  const int S = p.stages;
+  // a stage: [half][column][8 rows][128 bytes], MXFP4: then [half][K block][8 rows][16 bytes] of scales
+  const uint32_t half_bytes = uint32_t(p.box) * 1024u;
+  const uint32_t scale_copy = MX ? uint32_t(p.box) * 256u : 0u;  // of a half; stages stay 1024-byte aligned
+  const uint32_t scale_bytes = (scale_copy + 511u) & ~511u;
+  const uint32_t stage_bytes = 2u * (half_bytes + scale_bytes);
   auto full = [&](int s) { return base + p.off_bars + 8u * uint32_t(s); };
   auto empty = [&](int s) { return base + p.off_bars + 8u * uint32_t(S + s); };
   auto red_full = [&](int b) { return base + p.off_bars + 8u * uint32_t(2 * S + b); };
   auto red_empty = [&](int b) { return base + p.off_bars + 8u * uint32_t(2 * S + 2 + b); };
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + p.off_bars + 8 * (2 * S + 4));
-  int* finished = reinterpret_cast<int*>(smem + p.off_bars + 8 * (2 * S + 4) + 16);  // [1 + kMoeBatch]
   const MoeRoute route = moe_route_at(smem + p.off_route, p.T * p.top_k);
 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full(s), 1u);
-      mbar_init(empty(s), kMoeConsumers);
+      mbar_init(empty(s), kMoeConsumers / kMoeGroups);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(red_full(b), kMoeConsumers);
       mbar_init(red_empty(b), 1u);
     }
     *abort_flag = 0;
-    finished[0] = 0;
     fence_barrier_init();
   }
   if constexpr (GATE) {
     griddep_wait();
     griddep_launch_dependents();  // DOWN may start: what earlier kernels wrote is visible to it
-    for (int i = blockIdx.x * kMoeThreads + tid; i < p.H / 16; i += gridDim.x * kMoeThreads) p.counters[i] = 0;
   }
   // The routing tables (scratch: the ring, before its first copy).
   moe_route(p, route, reinterpret_cast<uint32_t*>(smem), 8 * NT);
 
+  if (GATE && blockIdx.x == 0)
+    for (int i = tid; i < p.T * p.top_k; i += kMoeThreads)
+      p.routed[i] = make_float2(route.weight[i], __int_as_float(route.expert[i]));
   const int chunks = route.totals[0];
   const int tiles = GATE ? p.I / 8 : p.H / 16, per_chunk = tiles * p.segments;
   const int K = GATE ? p.H : p.I;
   const int64_t units = int64_t(chunks) * per_chunk;
   const int u0 = int(units * blockIdx.x / gridDim.x), u1 = int(units * (blockIdx.x + 1) / gridDim.x);
   // A unit's place: chunk, K range, rows.
-  auto place = [&](int u, int& chunk, int& seg, int& tile) {
-    chunk = u / per_chunk;
-    const int rest = u - chunk * per_chunk;
-    seg = rest / tiles;
-    tile = rest - seg * tiles;
+  struct Place {
+    int chunk, seg, tile;
   };
-  const int stage_blocks = p.stage_row / BB;  // 128-wide blocks of a stage
+  const Place place0 = {u0 / per_chunk, u0 % per_chunk / tiles, u0 % per_chunk % tiles};
+  auto advance = [&](Place& at) {
+    if (++at.tile == tiles) {
+      at.tile = 0;
+      if (++at.seg == p.segments) at.seg = 0, ++at.chunk;
+    }
+  };
+  const int stage_blocks = p.box * (128 / BB);  // 128-wide K blocks of a stage
 
   if (warp == kMoeConsumers) {
     // ---------------------------------------------------------------- producer
-    const uint64_t policy = policy_evict_first(), scale_policy = policy_evict_normal();
-    int n = 0;
-    bool ok = true;
-    for (int u = u0; u < u1 && ok; ++u) {
-      int chunk, seg, tile;
-      place(u, chunk, seg, tile);
-      const int row = GATE ? (lane & 8 ? p.I : 0) + tile * 8 + (lane & 7) : tile * 16 + (lane & 15);
-      const uint8_t* src = p.w + int64_t(route.chunk_expert[chunk]) * p.w_expert + int64_t(row) * p.w_row +
-                           int64_t(seg) * p.seg_len / 128 * BB;
-      const int k_len = min(p.seg_len, K - seg * p.seg_len);
-      const int bytes = MX ? k_len / 2 : k_len;
-      for (int at = 0; at < bytes; at += p.stage_row, ++n) {
-        const int s = n % S;
-        if (n >= S) ok = mbar_wait(empty(s), uint32_t(n / S - 1) & 1u, abort_flag, kMoeWaitEmpty);
-        ok = __all_sync(~0u, ok);
-        if (!ok) break;
-        const uint32_t len = uint32_t(min(p.stage_row, bytes - at));
-        const int nb = (int(len) + BB - 1) / BB;
-        const uint32_t stage = base + uint32_t(s) * stage_bytes;
-        if (lane == 0) mbar_arrive_expect_tx(full(s), 16u * len + (MX ? uint32_t(nb) * 256u : 0u));
-        __syncwarp();
-        if (lane < 16) bulk_load(stage + uint32_t(lane * row_pitch), src + at, len, full(s), policy);
-        if constexpr (MX) {
-          // A block's scale words of 8 rows are 8 x 16 contiguous bytes of its
-          // tile, each with the words of the rows 32, 64 and 96 further on:
-          // a fourth of it is used here, the rest by the CTA's next units (from L2).
-          const int half = lane >> 4;  // rows 0-7 and 8-15 of the unit
-          const int r = GATE ? half * p.I + tile * 8 : tile * 16 + 8 * half;
-          const uint8_t* sc = static_cast<const uint8_t*>(p.ws) +
-                              ((int64_t(route.chunk_expert[chunk]) * p.rb + (r >> 7)) * p.kb + seg * (p.seg_len / 128) + at / BB) * 512 +
-                              (r & 31) * 16;
-          for (int i = lane & 15; i < nb; i += 16)
-            bulk_load(stage + uint32_t(16 * row_pitch + i * 256 + half * 128), sc + i * 512, 128u, full(s), scale_policy);
+    if (lane == 0) {
+      const uint64_t policy = policy_evict_first(), scale_policy = policy_evict_normal();
+      int n = 0, s = 0;
+      uint32_t phase = 1u;
+      bool ok = true;
+      Place at = place0;
+      for (int u = u0; u < u1 && ok; ++u, advance(at)) {
+        const int expert = route.chunk_expert[at.chunk];
+        const int row[2] = {GATE ? at.tile * 8 : at.tile * 16, GATE ? p.I + at.tile * 8 : at.tile * 16 + 8};
+        const int first = at.seg * (p.seg_len / 128) * BB / 128;  // 128-byte columns
+        const int last = first + (min(p.seg_len, K - at.seg * p.seg_len) * BB / 128 + 127) / 128;
+        for (int c = first; c < last; c += p.box, ++n) {
+          if (n >= S && !(ok = mbar_wait(empty(s), phase, abort_flag, kMoeWaitEmpty))) break;
+          const uint32_t to = base + uint32_t(s) * stage_bytes;
+          const int end = min(c + p.box, last);
+          if (end <= p.columns) {
+            mbar_arrive_expect_tx(full(s), 2u * (half_bytes + scale_copy));
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tma_load_4d(to + uint32_t(h) * half_bytes, &p.map_w, 0, row[h], c, expert, full(s), policy);
+          } else {  // the last column is short: column by column, zeros past the row
+            mbar_arrive_expect_tx(full(s), uint32_t(end - c) * 2048u + 2u * scale_copy);
+            for (int h = 0; h < 2; ++h)
+              for (int i = c; i < end; ++i)
+                tma_load_3d(to + uint32_t(h) * half_bytes + uint32_t(i - c) * 1024u, &p.map_tail, i * 128, row[h], expert,
+                            full(s), policy);
+          }
+          if constexpr (MX) {
+            // A K block's scale words of 8 rows are 128 contiguous bytes of
+            // its tile, each next to the words of the rows 32, 64 and 96
+            // further on: a fourth is used here, the rest by the units that
+            // follow (from L2).
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tma_load_4d(to + 2u * half_bytes + uint32_t(h) * scale_bytes, &p.map_s, (row[h] & 31) * 16, 2 * c, row[h] >> 7,
+                          expert, full(s), scale_policy);
+          }
+          if (++s == S) s = 0, phase ^= 1u;
         }
       }
+      for (int k = n > S ? n - S : 0; k < n; ++k) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMoeWaitDrain);
     }
-    for (int k = n > S ? n - S : 0; k < n; ++k) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMoeWaitDrain);
+    __syncwarp();
   } else if (warp < kMoeConsumers) {
     // ---------------------------------------------------------------- consumers
     const int g = lane >> 2, t4 = lane & 3;
+    // [32 values of K][token][lane quarter][16 bytes]; a column past the
+    // batch reads some other token's values and is not used
     uint8_t* bfrag = smem + p.off_b;
+    const uint32_t piece = uint32_t(p.cols) * 64u;
+    uint32_t b_lane[NT];
+#pragma unroll
+    for (int c = 0; c < NT; ++c) b_lane[c] = base + p.off_b + uint32_t(min(c * 8 + g, p.cols - 1) * 64 + t4 * 16);
     float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8 NT]
     if constexpr (!GATE) griddep_wait();                    // h
-    int n = 0, q = 0, have = -1, count = 0;
+    constexpr int kStep = kMoeConsumers / kMoeGroups;  // warps of a group
+    const int group = warp / kStep, warp_in_group = warp % kStep;
+    const uint32_t a_lane = ((lane >> 3) & 1) * half_bytes + (lane & 7) * 128u;
+    int have = -1, count = 0, s = 0, turn = 0;
+    uint32_t phase = 0u;
     bool ok = true;
     // Block FP8 scales: lane l holds those of K blocks l and l + 32 of the
-    // unit's two 8-row halves, requested a unit ahead.
-    float sc[2][2], sc_next[2][2];
-    auto load_scales = [&](int u, float (&v)[2][2]) {
-      int chunk, seg, tile;
-      place(u, chunk, seg, tile);
-      const float* e = static_cast<const float*>(p.ws) + int64_t(route.chunk_expert[chunk]) * p.rb * p.kb;
-      const int kb = seg * (p.seg_len / 128);
+    // unit's two 8-row halves, requested a unit ahead where they change.
+    float sc[2][2] = {}, sc_next[2][2] = {};
+    auto load_scales = [&](const Place& at) {
+      const float* e = static_cast<const float*>(p.ws) + int64_t(route.chunk_expert[at.chunk]) * p.rb * p.kb;
+      const int kb = at.seg * (p.seg_len / 128);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int r = GATE ? half * p.I + tile * 8 : tile * 16 + 8 * half;
+        const int r = GATE ? half * p.I + at.tile * 8 : at.tile * 16 + 8 * half;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int b = kb + lane + 32 * j;
-          v[half][j] = b < p.kb ? ldg_pinned(e + int64_t(r >> 7) * p.kb + b) : 0.f;
+          sc_next[half][j] = b < p.kb ? ldg_pinned(e + int64_t(r >> 7) * p.kb + b) : 0.f;
         }
       }
     };
-    if (!MX && u0 < u1) load_scales(u0, sc_next);
+    // Does a unit read the same block scales as the one before it?
+    auto same_scales = [&](const Place& at) {
+      return at.tile != 0 && (GATE ? (at.tile & 15) != 0 && ((p.I + at.tile * 8) & 127) != 0 : (at.tile & 7) != 0);
+    };
+    Place at = place0;
+    if (!MX && u0 < u1) load_scales(at);
     for (int u = u0; u < u1; ++u) {
-      int chunk, seg, tile;
-      place(u, chunk, seg, tile);
+      const int chunk = at.chunk, seg = at.seg, tile = at.tile;
+      advance(at);  // the next unit's
       if constexpr (!MX) {
 #pragma unroll
         for (int half = 0; half < 2; ++half) sc[half][0] = sc_next[half][0], sc[half][1] = sc_next[half][1];
-        if (u + 1 < u1) load_scales(u + 1, sc_next);
+        if (u + 1 < u1 && !same_scales(at)) load_scales(at);
       }
       const int k_len = min(p.seg_len, K - seg * p.seg_len);
       const int blocks = (k_len + 127) / 128;
@@ -497,15 +644,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
             uint32_t w[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v[2 * i] * to, v[2 * i + 1] * to);
-            const int nt = tok >> 3;
-            // 32 values of K make one 512-byte piece: [token of 8][lane quarter][16 bytes]
-            uint8_t* piece = bfrag + ((b * 4 + (l16 >> 2)) * NT + nt) * 512 + (tok & 7) * 64;
+            uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + tok * 64;
             if constexpr (MX) {
               // a lane's codes are 8 consecutive values
-              *reinterpret_cast<uint4*>(piece + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(to16 + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
               // a lane's codes are 4 consecutive values of each 16
-              uint8_t* at = piece + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
+              uint8_t* at = to16 + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
               *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
               *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
             }
@@ -514,98 +659,59 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
         }
         named_bar_sync(1, 32 * kMoeConsumers);
       }
+      // MXFP4: the 32-row quarter of the rows' scale tiles
+      const uint32_t word_a = uint32_t(((GATE ? tile * 8 : tile * 16) >> 5) & 3) * 4u;
+      const uint32_t word_b = scale_bytes + uint32_t(((GATE ? p.I + tile * 8 : tile * 16 + 8) >> 5) & 3) * 4u;
       float acc[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-      for (int b0 = 0; b0 < blocks; b0 += stage_blocks, ++n) {
-        const int s = n % S;
-        ok = mbar_wait(full(s), uint32_t(n / S) & 1u, abort_flag, kMoeWaitFull) && ok;
-        const int nb = min(stage_blocks, blocks - b0);
-        for (int i = (warp - q) & (kMoeConsumers - 1); i < nb; i += kMoeConsumers) {
-          const int b = b0 + i;  // block of this K range
-          float sa = 1.f, sb = 1.f;
-          float fa4[4], fb4[4];
-          if constexpr (MX) {
-            // the word of this row: 32-row quarter of its tile
-            const int ra = (GATE ? tile * 8 : tile * 16), rb = GATE ? p.I + tile * 8 : tile * 16 + 8;
-            const uint32_t at = base + uint32_t(s) * stage_bytes + uint32_t(16 * row_pitch + i * 256 + g * 16);
-            e8m0x4_to_float(ld_shared_u32(at + uint32_t((ra >> 5) & 3) * 4u), fa4);
-            e8m0x4_to_float(ld_shared_u32(at + 128u + uint32_t((rb >> 5) & 3) * 4u), fb4);
-          } else {
-            sa = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][1], b & 31);
-            sb = GATE ? __shfl_sync(~0u, b < 32 ? sc[1][0] : sc[1][1], b & 31) : sa;
-          }
-          // ldmatrix rows: lanes 0-7 / 8-15 the two row halves of one 16-byte
-          // column, lanes 16-31 of the next
-          const uint32_t a_addr = base + uint32_t(s) * stage_bytes + uint32_t((lane & 15) * row_pitch + i * BB + (lane >> 4) * 16);
-          const uint8_t* bp = bfrag + b * 4 * NT * 512 + lane * 16;
-          const int pairs = min(4, (k_len - b * 128) / 32);  // 32-wide steps of the block
-          float part[NT][4];
-#pragma unroll
-          for (int c = 0; c < NT; ++c) part[c][0] = part[c][1] = part[c][2] = part[c][3] = 0.f;
-          if constexpr (MX) {
-#pragma unroll
-            for (int pp = 0; pp < 4; pp += 2) {
-              if (pp < pairs) {
-                uint32_t r[4];
-                ldmatrix_x4(a_addr + uint32_t(pp * 16), r);
-#pragma unroll
-                for (int h2 = 0; h2 < 2; ++h2) {
-                  if (pp + h2 < pairs) {
-                    uint32_t ha[4], hb[4];
-                    e2m1x8_to_f16(r[2 * h2], ha);
-                    e2m1x8_to_f16(r[2 * h2 + 1], hb);
-                    const float fa = fa4[pp + h2], fb = fb4[pp + h2];
-#pragma unroll
-                    for (int c = 0; c < NT; ++c) {
-                      if (c == 0 || c * 8 < count) {
-                        const uint4 bv = *reinterpret_cast<const uint4*>(bp + ((pp + h2) * NT + c) * 512);
-                        float d[4] = {0.f, 0.f, 0.f, 0.f};
-                        mma_f16(d, ha[0], hb[0], ha[1], hb[1], bv.x, bv.y);
-                        mma_f16(d, ha[2], hb[2], ha[3], hb[3], bv.z, bv.w);
-                        part[c][0] = fmaf(d[0], fa, part[c][0]);
-                        part[c][1] = fmaf(d[1], fa, part[c][1]);
-                        part[c][2] = fmaf(d[2], fb, part[c][2]);
-                        part[c][3] = fmaf(d[3], fb, part[c][3]);
-                      }
-                    }
-                  }
-                }
-              }
+      for (int b0 = 0; b0 < blocks; b0 += stage_blocks) {
+        const bool mine = turn == group;
+        if (++turn == kMoeGroups) turn = 0;
+        if (mine) {
+          ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
+          const int nb = min(stage_blocks, blocks - b0);
+          const uint32_t stage = base + uint32_t(s) * stage_bytes;
+          // One 128-wide K block: its scales of rows g and g + 8, this lane's
+          // ldmatrix row (lanes 0-7 / 8-15 the two halves' rows in one 16-byte
+          // chunk, lanes 16-31 in the next), its token fragments and scales.
+          auto block = [&](int i, auto full_tag, int steps) {
+            constexpr bool FULL = decltype(full_tag)::value;
+            const int b = b0 + i;
+            float fa[4], fb[4];
+            if constexpr (MX) {
+              const uint32_t word = stage + 2u * half_bytes + uint32_t(i * 128 + g * 16);
+              e8m0x4_to_float(ld_shared_u32(word + word_a), fa);
+              e8m0x4_to_float(ld_shared_u32(word + word_b), fb);
+            } else {
+              fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][1], b & 31);
+              fb[0] = GATE ? __shfl_sync(~0u, b < 32 ? sc[1][0] : sc[1][1], b & 31) : fa[0];
             }
-          } else {
+            const uint32_t a_row = stage + a_lane + uint32_t(MX ? i >> 1 : i) * 1024u;
+            const uint32_t chunk0 = (MX ? (i & 1) * 4u : 0u) + (lane >> 4);
+            uint32_t b_addr[NT];
 #pragma unroll
-            for (int pp = 0; pp < 4; ++pp) {
-              if (pp < pairs) {
-                uint32_t r[4], lo[4], hi[4];
-                ldmatrix_x4(a_addr + uint32_t(pp * 32), r);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) e4m3x4_to_f16(r[k], lo[k], hi[k]);
-#pragma unroll
-                for (int c = 0; c < NT; ++c) {
-                  if (c == 0 || c * 8 < count) {
-                    const uint4 bv = *reinterpret_cast<const uint4*>(bp + (pp * NT + c) * 512);
-                    mma_f16(part[c], lo[0], lo[1], hi[0], hi[1], bv.x, bv.y);
-                    mma_f16(part[c], lo[2], lo[3], hi[2], hi[3], bv.z, bv.w);
-                  }
-                }
-              }
-            }
+            for (int c = 0; c < NT; ++c) b_addr[c] = b_lane[c] + uint32_t(b * 4) * piece;
+            const float* tsb = ts + b * 8 * NT + 2 * t4;
+            if (NT == 1 || count <= 8) moe_block<Cfg, 1, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
+            else moe_block<Cfg, NT, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
+          };
+          // Whole blocks two at a time (their loads and MMA chains overlap),
+          // then what is left; the last block of K may be short.
+          const int whole = min(nb, (k_len - b0 * 128) / 128);
+          int i = warp_in_group;
+          for (; i + kStep < whole; i += 2 * kStep) {
+            block(i, std::true_type(), 4);
+            block(i + kStep, std::true_type(), 4);
           }
-#pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            if (c == 0 || c * 8 < count) {
-              const float2 tsc = *reinterpret_cast<const float2*>(ts + b * 8 * NT + c * 8 + 2 * t4);
-              acc[c][0] = fmaf(part[c][0], tsc.x * sa, acc[c][0]);
-              acc[c][1] = fmaf(part[c][1], tsc.y * sa, acc[c][1]);
-              acc[c][2] = fmaf(part[c][2], tsc.x * sb, acc[c][2]);
-              acc[c][3] = fmaf(part[c][3], tsc.y * sb, acc[c][3]);
-            }
+          for (; i < nb; i += kStep) {
+            if (i < whole) block(i, std::true_type(), 4);
+            else block(i, std::false_type(), (k_len - (b0 + i) * 128) / 32);
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(empty(s));
         }
-        q += nb;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty(s));
+        if (++s == S) s = 0, phase ^= 1u;
       }
       // ---- this warp's sums of the unit
       const int i = u - u0, buf = i & 1;
@@ -619,17 +725,13 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
   } else {
     // ---------------------------------------------------------------- finisher
     const int g = lane >> 2, t4 = lane & 3;
-    if constexpr (!GATE) griddep_wait();  // the counters, y
-    const bool none = !GATE && units == 0;
-    if (none) {  // no pair has an expert: y = 0
-      T* y = static_cast<T*>(p.y);
-      for (int64_t i = int64_t(blockIdx.x) * 32 + lane; i < int64_t(p.T) * p.H; i += int64_t(gridDim.x) * 32)
-        y[i / p.H * p.ldy + i % p.H] = T(0.f);
+    if constexpr (!GATE) {
+      griddep_wait();  // z
+      griddep_launch_dependents();
     }
-    int flushed = u0;  // units whose arrival is counted
-    for (int u = u0; u < u1; ++u) {
-      int chunk, seg, tile;
-      place(u, chunk, seg, tile);
+    Place at = place0;
+    for (int u = u0; u < u1; ++u, advance(at)) {
+      const int chunk = at.chunk, seg = at.seg, tile = at.tile;
       const int i = u - u0, buf = i & 1;
       if (!mbar_wait(red_full(buf), uint32_t(i / 2) & 1u, abort_flag, kMoeWaitRedFull)) break;
       const int count = route.chunk_count[chunk], first = route.chunk_first[chunk];
@@ -660,34 +762,7 @@ __global__ void __launch_bounds__(kMoeThreads, 1) moe_kernel(const __grid_consta
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(red_empty(buf));
-      if constexpr (!GATE) {
-        // Arrivals are counted a batch of units at a time: a fence and an
-        // atomic cost as much as streaming two to four units.
-        if (u + 1 - flushed == kMoeBatch || u + 1 == u1) {
-          __threadfence();
-          __syncwarp();
-          bool last = false;
-          int tile_l = 0;
-          if (lane < u + 1 - flushed) {
-            int c_l, s_l;
-            place(flushed + lane, c_l, s_l, tile_l);
-            last = atomicAdd(p.counters + tile_l, 1) == chunks * p.segments - 1;
-          }
-          __threadfence();
-          const uint32_t lasts = __ballot_sync(~0u, last);
-          if (last) finished[1 + __popc(lasts & ((1u << lane) - 1u))] = tile_l;
-          if (lane == 0) finished[0] = __popc(lasts);
-          __syncwarp();
-          flushed = u + 1;
-          if (u + 1 < u1) moe_combine<T>(p, route, finished, lane, 32);
-        }
-      }
     }
-  }
-  if constexpr (!GATE) {
-    __syncthreads();
-    // the last batch's row tiles, by every warp
-    if (!*abort_flag) moe_combine<T>(p, route, finished, tid, kMoeThreads);
   }
 }
 
