@@ -95,29 +95,29 @@ int round_up(int x, int m) { return cdiv(x, m) * m; }
 // How one kernel's units (segments of seg_len values of K) and shared memory
 // are laid out.
 struct MoeLayout {
-  int segments, seg_len, box, stages, smem;
+  int segments, seg_len, box, stages, smem, cols, resident;
   uint32_t off_b, off_ts, off_red, off_route, off_bars;
 };
 
-// K of `k` values in `segments` ranges; as many stages as fit beside a range's
-// activations, in half an SM's shared memory where four do -- DOWN then starts
-// beside GATE and requests its weights while GATE runs -- else in all of it.
-bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int nt, MoeLayout* out) {
+// K of `k` values in `segments` ranges, `entries` tokens or pairs that could
+// have a column of their own, within `limit` bytes of shared memory.
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int nt, int warps, int limit, int min_stages,
+                MoeLayout* out) {
   const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
   const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, 8);
   out->box = cdiv(columns, unit_stages);
   out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
   out->segments = cdiv(k, out->seg_len);
+  out->resident = entries <= 8 * nt;
+  out->cols = out->resident ? entries : std::min(P, 8 * nt);
   const int blocks = cdiv(std::min(k, out->seg_len), 128);
   const int stage = round_up(out->box * (2048 + (p.format ? 512 : 0)), 1024);
-  const int b = blocks * 256 * std::min(p.T, 8 * nt), ts = round_up(blocks * 8 * nt * 4, 16);
-  const int red = 2 * kMoeConsumers * nt * 512, route = round_up(moe_route_bytes(P), 16);
+  const int b = blocks * 256 * out->cols, ts = round_up(blocks * 8 * nt * 4, 16);
+  const int red = (warps * nt >= 32 ? 1 : 2) * warps * nt * 512, route = round_up(moe_route_bytes(P), 16);
   const int scratch = P > 32 ? p.E * (cdiv(P, 32) + 1) * 4 : 0;
   auto end_of = [&](int stages) { return 8 * (2 * stages + 4) + 16; };
-  const int fixed = 1024 + b + ts + red + route + end_of(16);
-  int stages = std::min(16, (kMoeHalfSmem - fixed) / stage);
-  if (stages < 4 || stages * stage < scratch) stages = std::min(16, (kMaxSmem - fixed) / stage);
-  if (stages < kMoeMinStages || stages * stage < scratch) return false;
+  const int stages = std::min(16, (limit - (1024 + b + ts + red + route + end_of(16))) / stage);
+  if (stages < min_stages || stages * stage < scratch) return false;
   out->stages = stages;
   out->off_b = uint32_t(stages * stage);
   out->off_ts = out->off_b + uint32_t(b);
@@ -129,16 +129,25 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int nt, MoeLayou
 }
 
 struct MoeShape {
-  int nt;  // 8-token tiles of a chunk
+  int nt, warps;  // 8-token tiles of a chunk; consumer warps
   MoeLayout gate, down;
 };
 
-// Tokens of a chunk: 16 where the batch can fill them and the activations of
-// both kernels leave room for the ring, else 8.
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
-  for (s->nt = p.T > 8 ? 2 : 1; s->nt >= 1; --s->nt)
-    if (moe_layout(p, p.H, 1, s->nt, &s->gate) && moe_layout(p, p.I, cdiv(p.I, kMoeSegment), s->nt, &s->down)) return true;
-  return false;
+  const int P = p.T * p.top_k, segments = cdiv(p.I, kMoeSegment);
+  auto fits = [&](int nt, int warps, int limit, int min_stages) {
+    s->nt = nt;
+    s->warps = warps;
+    return moe_layout(p, p.H, 1, p.T, nt, warps, limit, min_stages, &s->gate) &&
+           moe_layout(p, p.I, segments, P, nt, warps, limit, min_stages, &s->down);
+  };
+  // Up to 8 tokens: both kernels in half an SM's shared memory, so that DOWN
+  // starts beside GATE and requests its weights while GATE runs.
+  if (p.T <= 8 && fits(1, 8, kMoeHalfSmem, 4)) return true;
+  // Chunks of 16 where experts have more than four tokens on average, else of
+  // 8: a ring twice as deep, and few experts are read twice.
+  if (p.T > 8 && P > 4 * p.E && fits(2, 16, kMaxSmem, kMoeMinStages)) return true;
+  return fits(1, 16, kMaxSmem, kMoeMinStages);
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
@@ -146,6 +155,7 @@ int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int
              const void* scales, int E, int rows, int k) {
   const uint64_t bytes = uint64_t(format ? k / 2 : k), full = bytes / 128;
   mp.columns = int(full);
+  mp.rows = rows;
   if (E == 1) w_expert = w_row * rows;  // one expert's stride says nothing
   auto fn = encode_fn();
   if (!fn) return fail(BFP8_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
@@ -158,8 +168,12 @@ int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int
     if (r != CUDA_SUCCESS) return fail(BFP8_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
     return int(BFP8_OK);
   };
-  if (full > 0) {  // [128 bytes][rows][columns][experts]
-    const cuuint64_t dims[4] = {128, cuuint64_t(rows), full, cuuint64_t(E)};
+  // A short last column may be read past a row's end where another row of the
+  // stack follows in memory.
+  mp.tail_reads_on = bytes % 128 != 0 && w_expert >= w_row * rows;
+  const uint64_t columns = full + (mp.tail_reads_on ? 1 : 0);
+  if (columns > 0) {  // [128 bytes][rows][columns][experts]
+    const cuuint64_t dims[4] = {128, cuuint64_t(rows), columns, cuuint64_t(E)};
     const cuuint64_t strides[3] = {cuuint64_t(w_row), 128, cuuint64_t(w_expert)};
     const cuuint32_t box[4] = {128, 8, cuuint32_t(lay.box), 1};
     if (int r = encode(&mp.map_w, w, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return r;
@@ -220,10 +234,11 @@ int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms,
   mp.off_red = lay.off_red;
   mp.off_route = lay.off_route;
   mp.off_bars = lay.off_bars;
-  mp.cols = std::min(mp.T, 8 * Cfg::NT);
+  mp.cols = lay.cols;
+  mp.resident = lay.resident;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(num_sms));
-  cfg.blockDim = dim3(kMoeThreads);
+  cfg.blockDim = dim3(Cfg::THREADS);
   cfg.dynamicSmemBytes = size_t(lay.smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -235,19 +250,23 @@ int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms,
 }
 
 template <bool GATE>
-int launch_moe_any(MoeParams& mp, const MoeLayout& lay, int format, int nt, int x_type, int dev, int num_sms,
+int launch_moe_any(MoeParams& mp, const MoeLayout& lay, int format, const MoeShape& s, int x_type, int dev, int num_sms,
                    cudaStream_t stream) {
-  auto go = [&](auto mx, auto tiles, auto t) {
-    return launch_moe_kernel<MoeCfg<GATE, decltype(mx)::value, decltype(tiles)::value, decltype(t)>>(mp, lay, dev,
-                                                                                                     num_sms, stream);
+  auto go = [&](auto mx, auto tiles, auto warps, auto t) {
+    return launch_moe_kernel<MoeCfg<GATE, decltype(mx)::value, decltype(tiles)::value, decltype(warps)::value, decltype(t)>>(
+        mp, lay, dev, num_sms, stream);
   };
-  auto by_type = [&](auto mx, auto tiles) {
-    return x_type == 1 ? go(mx, tiles, __nv_bfloat16()) : go(mx, tiles, __half());
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using W8 = std::integral_constant<int, 8>;
+  using W16 = std::integral_constant<int, 16>;
+  auto by_type = [&](auto mx, auto tiles, auto warps) {
+    return x_type == 1 ? go(mx, tiles, warps, __nv_bfloat16()) : go(mx, tiles, warps, __half());
   };
-  auto by_tiles = [&](auto mx) {
-    return nt == 1 ? by_type(mx, std::integral_constant<int, 1>()) : by_type(mx, std::integral_constant<int, 2>());
+  auto by_shape = [&](auto mx) {
+    return s.nt == 2 ? by_type(mx, Two(), W16()) : s.warps == 16 ? by_type(mx, One(), W16()) : by_type(mx, One(), W8());
   };
-  return format ? by_tiles(std::true_type()) : by_tiles(std::false_type());
+  return format ? by_shape(std::true_type()) : by_shape(std::false_type());
 }
 
 }  // namespace
@@ -370,9 +389,9 @@ int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
   mp.top_k = p.top_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (int r = moe_maps(mp, s.gate, p.format, p.w13, p.w13_expert, p.w13_row, p.s13, p.E, 2 * p.I, p.H)) return r;
-  if (int r = launch_moe_any<true>(mp, s.gate, p.format, s.nt, p.x_type, dev, num_sms, st)) return r;
+  if (int r = launch_moe_any<true>(mp, s.gate, p.format, s, p.x_type, dev, num_sms, st)) return r;
   if (int r = moe_maps(mp, s.down, p.format, p.w2, p.w2_expert, p.w2_row, p.s2, p.E, p.H, p.I)) return r;
-  if (int r = launch_moe_any<false>(mp, s.down, p.format, s.nt, p.x_type, dev, num_sms, st)) return r;
+  if (int r = launch_moe_any<false>(mp, s.down, p.format, s, p.x_type, dev, num_sms, st)) return r;
   const MoeSumParams sp{mp.z, mp.routed, p.y, p.ldy, p.T, p.H, p.top_k, s.down.segments};
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(cdiv(p.T * (p.H / 4), kMoeSumThreads)));

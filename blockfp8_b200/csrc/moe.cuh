@@ -23,8 +23,8 @@
 //   bytes, 1 expert] in the 128-byte swizzle, which ldmatrix reads without
 //   conflicts.  (One bulk copy per row took the issuing warp about 60 clocks
 //   each, 1,000 a stage: more than the 700 that HBM takes to deliver it.)
-// - Eight consumer warps in two groups take stages in turn, and the 128-wide K
-//   blocks of a stage in turn inside a group:
+// - Consumer warps (8 or 16) in groups of four take stages in turn, and the
+//   128-wide K blocks of a stage in turn inside a group:
 //   ldmatrix, codes to f16 (exact: cvt, 128 codes per clock and SM), mma.sync
 //   m16n8k16 with fp32 accumulation, then the block's scales in fp32.  The
 //   legacy MMA is no bound here (one 8-token MMA per 256 weights is 0.09 of
@@ -34,13 +34,13 @@
 //   one power-of-two scale per token and 128 values, which puts the largest
 //   at 2^14: bf16 values are exact down to 2^-28 of it, and h (fp32) keeps 11
 //   bits, 8 times finer than a bf16 h would.
-// - A last warp finishes units: it adds the eight warps' sums in warp order.
+// - A last warp finishes units: it adds the consumers' sums in warp order.
 //   z goes to memory and a small third kernel adds each token's pairs in j
 //   order.  (Counting arrivals and letting the last unit of an output row tile
 //   add them makes the slowest CTA do nearly all of it: 2.4 times the median
 //   CTA's time at 64 tokens.)  No result depends on the order of arrival.
 //
-// Warps: 0-7 consumers, 8 producer, 9 finisher.
+// Warps: consumers, then the producer, then the finisher.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -58,9 +58,7 @@ namespace bfp8 {
 constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxExperts = 512;
-constexpr int kMoeConsumers = 8;  // warps, in groups that take stages in turn
-constexpr int kMoeGroups = 2;
-constexpr int kMoeThreads = 32 * (kMoeConsumers + 2);
+constexpr int kMoeGroupWarps = 4;  // consumer warps of a group; groups take stages in turn
 
 struct MoeParams {
   const void* x;  // [T, H] bf16 or fp16
@@ -75,7 +73,7 @@ struct MoeParams {
   // This kernel's weights, rows of `columns` full 128-byte columns (map_w: 8
   // rows x box columns) and perhaps one shorter (map_tail: 8 rows x 128 bytes).
   CUtensorMap map_w, map_tail;
-  int columns;
+  int columns, rows, tail_reads_on;
   CUtensorMap map_s;  // MXFP4: scale tiles, [128 bytes = 8 rows] x 2 box K blocks
   const void* ws;     // block FP8: scales fp32 [E, rb, kb]
   int rb, kb;
@@ -85,7 +83,8 @@ struct MoeParams {
   int T, H, I, E, top_k;
   int segments, seg_len;  // K ranges of DOWN
   int stages, box;        // ring: stages, 128-byte columns of a stage
-  int cols;               // token columns held: min(T, 8 NT)
+  int cols;               // token columns held
+  int resident;           // every token (GATE) or pair (DOWN) has its own
   uint32_t off_b, off_ts, off_red, off_route, off_bars;  // shared memory
 };
 
@@ -193,27 +192,35 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, const MoeRoute& r,
   }
 }
 
-// The router and the chunk tables, by all threads of the CTA.  scratch: room
-// for E (ceil(P / 32) + 1) words.
-__device__ void moe_route(const MoeParams& p, const MoeRoute& r, uint32_t* scratch, int cap) {
+// Each pair's expert and weight.  Tokens go to warps from the last one down:
+// the first ones have other work at that time.
+template <int THREADS>
+__device__ __forceinline__ void moe_select(const MoeParams& p, const MoeRoute& r) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int P = p.T * p.top_k, words = (P + 31) / 32;
-  uint32_t* masks = scratch;                                     // [E][words] pairs of each expert
-  int* offsets = reinterpret_cast<int*>(scratch + p.E * words);  // [E]
-  if (P > 32)
-    for (int i = tid; i < p.E * words; i += kMoeThreads) masks[i] = 0u;
   if (p.logits) {
-    for (int t = warp; t < p.T; t += kMoeThreads / 32) {
+    for (int t = THREADS / 32 - 1 - warp; t < p.T; t += THREADS / 32) {
       if (p.E <= 128) moe_top_k<4>(p, r, t, lane);
       else moe_top_k<kMoeMaxExperts / 32>(p, r, t, lane);
     }
   } else {
-    for (int i = tid; i < P; i += kMoeThreads) {
+    for (int i = tid; i < p.T * p.top_k; i += THREADS) {
       const int e = p.ids[i];
       r.expert[i] = short(e >= 0 && e < p.E ? e : -1);
       r.weight[i] = p.weights[i];
     }
   }
+}
+
+// The chunk tables, by all threads of the CTA; at most cap pairs a chunk.
+// scratch: room for E (ceil(P / 32) + 1) words.
+template <int THREADS>
+__device__ __forceinline__ void moe_group(const MoeParams& p, const MoeRoute& r, uint32_t* scratch, int cap) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int P = p.T * p.top_k, words = (P + 31) / 32;
+  uint32_t* masks = scratch;                                     // [E][words] pairs of each expert
+  int* offsets = reinterpret_cast<int*>(scratch + p.E * words);  // [E]
+  if (P > 32)
+    for (int i = tid; i < p.E * words; i += THREADS) masks[i] = 0u;
   __syncthreads();
   if (P <= 32) {
     // One warp, a pair a lane; an expert's chunks stand where its first pair does.
@@ -240,12 +247,12 @@ __device__ void moe_route(const MoeParams& p, const MoeRoute& r, uint32_t* scrat
       }
     }
   } else {
-    for (int i = tid; i < P; i += kMoeThreads) {
+    for (int i = tid; i < P; i += THREADS) {
       const int e = r.expert[i];
       if (e >= 0) atomicOr(masks + e * words + i / 32, 1u << (i & 31));
     }
     __syncthreads();
-    for (int e = tid; e < p.E; e += kMoeThreads) {
+    for (int e = tid; e < p.E; e += THREADS) {
       int n = 0;
       for (int w = 0; w < words; ++w) n += __popc(masks[e * words + w]);
       offsets[e] = n;
@@ -268,7 +275,7 @@ __device__ void moe_route(const MoeParams& p, const MoeRoute& r, uint32_t* scrat
       if (lane == 0) r.totals[0] = chunks;
     }
     __syncthreads();
-    for (int e = tid; e < p.E; e += kMoeThreads) {
+    for (int e = tid; e < p.E; e += THREADS) {
       const int first = offsets[e] >> 16, chunk = offsets[e] & 0xFFFF;
       int n = 0;
       for (int w = 0; w < words; ++w) {
@@ -372,10 +379,15 @@ __global__ void __launch_bounds__(kMoeSumThreads) moe_sum_kernel(const MoeSumPar
   *reinterpret_cast<uint2*>(static_cast<T*>(p.y) + int64_t(t) * p.ldy + col) = out;
 }
 
-template <bool GATE_, bool MX_, int NT_, class T_>
+template <bool GATE_, bool MX_, int NT_, int WARPS_, class T_>
 struct MoeCfg {
   static constexpr bool GATE = GATE_, MX = MX_;
-  static constexpr int NT = NT_;  // 8-token MMA tiles of a chunk
+  static constexpr int NT = NT_;        // 8-token MMA tiles of a chunk
+  static constexpr int WARPS = WARPS_;  // consumers
+  static constexpr int GROUPS = WARPS / kMoeGroupWarps;
+  static constexpr int THREADS = 32 * (WARPS + 2);
+  static constexpr int RED_BUFS = WARPS * NT >= 32 ? 1 : 2;  // buffers of the warps' sums (512 NT bytes a warp)
+  static constexpr int CTAS_PER_SM = WARPS == 8 ? 2 : 1;
   using T = T_;                   // x and y
   static constexpr int BLOCK_BYTES = MX ? 64 : 128;  // 128 values of K of one row
 };
@@ -456,9 +468,10 @@ __device__ __forceinline__ void moe_block(float (&acc)[Cfg::NT][4], uint32_t a_r
 }
 
 template <class Cfg>
-__global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(const __grid_constant__ MoeParams p) {
+__global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(const __grid_constant__ MoeParams p) {
   constexpr bool GATE = Cfg::GATE, MX = Cfg::MX;
-  constexpr int NT = Cfg::NT, BB = Cfg::BLOCK_BYTES;
+  constexpr int NT = Cfg::NT, BB = Cfg::BLOCK_BYTES, W = Cfg::WARPS, RB = Cfg::RED_BUFS;
+  constexpr int THREADS = Cfg::THREADS;
   using T = typename Cfg::T;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -480,10 +493,10 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
       mbar_init(full(s), 1u);
-      mbar_init(empty(s), kMoeConsumers / kMoeGroups);
+      mbar_init(empty(s), kMoeGroupWarps);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(red_full(b), kMoeConsumers);
+      mbar_init(red_full(b), W);
       mbar_init(red_empty(b), 1u);
     }
     *abort_flag = 0;
@@ -493,11 +506,61 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
     griddep_wait();
     griddep_launch_dependents();  // DOWN may start: what earlier kernels wrote is visible to it
   }
-  // The routing tables (scratch: the ring, before its first copy).
-  moe_route(p, route, reinterpret_cast<uint32_t*>(smem), 8 * NT);
+  // Activations in shared memory as f16 in MMA fragment order,
+  // [32 values of K][token column][lane quarter][16 bytes], and one power of
+  // two per column and 128-wide block.  A column past the batch reads some
+  // other token's values and is not used.
+  uint8_t* bfrag = smem + p.off_b;
+  float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8 NT]
+  const uint32_t piece = uint32_t(p.cols) * 64u;
+  auto fragments = [&](int columns, int k_len, auto row_of) {  // by the consumer warps
+    const int blocks = (k_len + 127) / 128, tasks = columns * blocks;
+    const int half = tid >> 4, l16 = tid & 15;  // a half-warp's task is one column's block
+    for (int task0 = 0; task0 < tasks; task0 += 2 * W) {
+      const int task = task0 + half;
+      const int col = task / blocks, b = task - col * blocks;
+      const int k = b * 128 + l16 * 8;
+      float v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      if (task < tasks && k < k_len) load8(row_of(col) + k, v);
+      uint32_t m = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+      float to, back;
+      moe_act_scale(m, to, back);
+      if (task < tasks) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v[2 * i] * to, v[2 * i + 1] * to);
+        uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + col * 64;
+        if constexpr (MX) {
+          // a lane's codes are 8 consecutive values
+          *reinterpret_cast<uint4*>(to16 + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+          // a lane's codes are 4 consecutive values of each 16
+          uint8_t* at = to16 + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
+          *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+          *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
+        }
+        if (l16 == 0) ts[b * 8 * NT + col] = back;
+      }
+    }
+  };
+
+  // Resident: all tokens (GATE) or pairs (DOWN) have a column of their own, laid
+  // out once, and a chunk uses its pairs' columns; else a chunk's pairs are laid
+  // out when a unit of it comes up.
+  moe_select<THREADS>(p, route);
+  if (GATE && p.resident && warp < W)
+    fragments(p.T, p.H, [&](int t) { return static_cast<const T*>(p.x) + int64_t(t) * p.ldx; });
+  // (scratch: the ring, before its first copy)
+  moe_group<THREADS>(p, route, reinterpret_cast<uint32_t*>(smem), p.resident ? p.T * p.top_k : p.cols);
 
   if (GATE && blockIdx.x == 0)
-    for (int i = tid; i < p.T * p.top_k; i += kMoeThreads)
+    for (int i = tid; i < p.T * p.top_k; i += THREADS)
       p.routed[i] = make_float2(route.weight[i], __int_as_float(route.expert[i]));
   const int chunks = route.totals[0];
   const int tiles = GATE ? p.I / 8 : p.H / 16, per_chunk = tiles * p.segments;
@@ -517,7 +580,7 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
   };
   const int stage_blocks = p.box * (128 / BB);  // 128-wide K blocks of a stage
 
-  if (warp == kMoeConsumers) {
+  if (warp == W) {
     // ---------------------------------------------------------------- producer
     if (lane == 0) {
       const uint64_t policy = policy_evict_first(), scale_policy = policy_evict_normal();
@@ -534,12 +597,15 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
           if (n >= S && !(ok = mbar_wait(empty(s), phase, abort_flag, kMoeWaitEmpty))) break;
           const uint32_t to = base + uint32_t(s) * stage_bytes;
           const int end = min(c + p.box, last);
-          if (end <= p.columns) {
+          // A short last column is read past the row's end, into the next
+          // row: consumers stop at K.  Behind the stack's last row there may
+          // be nothing to read.
+          if (end <= p.columns || (p.tail_reads_on && (expert < p.E - 1 || max(row[0], row[1]) + 8 < p.rows))) {
             mbar_arrive_expect_tx(full(s), 2u * (half_bytes + scale_copy));
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               tma_load_4d(to + uint32_t(h) * half_bytes, &p.map_w, 0, row[h], c, expert, full(s), policy);
-          } else {  // the last column is short: column by column, zeros past the row
+          } else {  // column by column, zeros past the row
             mbar_arrive_expect_tx(full(s), uint32_t(end - c) * 2048u + 2u * scale_copy);
             for (int h = 0; h < 2; ++h)
               for (int i = c; i < end; ++i)
@@ -562,19 +628,14 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
       for (int k = n > S ? n - S : 0; k < n; ++k) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMoeWaitDrain);
     }
     __syncwarp();
-  } else if (warp < kMoeConsumers) {
+  } else if (warp < W) {
     // ---------------------------------------------------------------- consumers
     const int g = lane >> 2, t4 = lane & 3;
-    // [32 values of K][token][lane quarter][16 bytes]; a column past the
-    // batch reads some other token's values and is not used
-    uint8_t* bfrag = smem + p.off_b;
-    const uint32_t piece = uint32_t(p.cols) * 64u;
     uint32_t b_lane[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c) b_lane[c] = base + p.off_b + uint32_t(min(c * 8 + g, p.cols - 1) * 64 + t4 * 16);
-    float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8 NT]
-    if constexpr (!GATE) griddep_wait();                    // h
-    constexpr int kStep = kMoeConsumers / kMoeGroups;  // warps of a group
+    if constexpr (!GATE) griddep_wait();  // h
+    constexpr int kStep = kMoeGroupWarps;
     const int group = warp / kStep, warp_in_group = warp % kStep;
     const uint32_t a_lane = ((lane >> 3) & 1) * half_bytes + (lane & 7) * 128u;
     int have = -1, count = 0, s = 0, turn = 0;
@@ -612,52 +673,19 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
       }
       const int k_len = min(p.seg_len, K - seg * p.seg_len);
       const int blocks = (k_len + 127) / 128;
-      if (have != chunk * p.segments + seg) {
-        // ---- the chunk's activations to f16 fragments
-        have = chunk * p.segments + seg;
-        count = route.chunk_count[chunk];
-        named_bar_sync(1, 32 * kMoeConsumers);
-        const int half = tid >> 4, l16 = tid & 15;  // 16 half-warps; a task is one token's block
-        const int tasks = count * blocks;
-        for (int task0 = 0; task0 < tasks; task0 += 16) {
-          const int task = task0 + half;
-          const int tok = task / blocks, b = task - tok * blocks;
-          const int k = b * 128 + l16 * 8;
-          float v[8];
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0.f;
-          if (task < tasks && k < k_len) {
-            const int pair = route.list[route.chunk_first[chunk] + tok];
-            if constexpr (GATE)
-              load8(static_cast<const T*>(p.x) + int64_t(pair / p.top_k) * p.ldx + k, v);
-            else
-              load8(p.h + int64_t(pair) * p.I + seg * p.seg_len + k, v);
-          }
-          uint32_t m = 0u;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
-          float to, back;
-          moe_act_scale(m, to, back);
-          if (task < tasks) {
-            uint32_t w[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v[2 * i] * to, v[2 * i + 1] * to);
-            uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + tok * 64;
-            if constexpr (MX) {
-              // a lane's codes are 8 consecutive values
-              *reinterpret_cast<uint4*>(to16 + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
-              // a lane's codes are 4 consecutive values of each 16
-              uint8_t* at = to16 + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
-              *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-              *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
-            }
-            if (l16 == 0) ts[b * 8 * NT + tok] = back;
-          }
+      const int key = p.resident ? seg : chunk * p.segments + seg;
+      if (have != key) {
+        count = p.resident ? p.cols : route.chunk_count[chunk];
+        if (!GATE || !p.resident) {
+          named_bar_sync(1, 32 * W);  // every warp is done with the last ones
+          fragments(count, k_len, [&](int col) {
+            const int pair = p.resident ? col : route.list[route.chunk_first[chunk] + col];
+            if constexpr (GATE) return static_cast<const T*>(p.x) + int64_t(pair / p.top_k) * p.ldx;
+            else return p.h + int64_t(pair) * p.I + seg * p.seg_len;
+          });
+          named_bar_sync(1, 32 * W);
         }
-        named_bar_sync(1, 32 * kMoeConsumers);
+        have = key;
       }
       // MXFP4: the 32-row quarter of the rows' scale tiles
       const uint32_t word_a = uint32_t(((GATE ? tile * 8 : tile * 16) >> 5) & 3) * 4u;
@@ -667,7 +695,7 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
       for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
       for (int b0 = 0; b0 < blocks; b0 += stage_blocks) {
         const bool mine = turn == group;
-        if (++turn == kMoeGroups) turn = 0;
+        if (++turn == Cfg::GROUPS) turn = 0;
         if (mine) {
           ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
           const int nb = min(stage_blocks, blocks - b0);
@@ -714,9 +742,9 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
         if (++s == S) s = 0, phase ^= 1u;
       }
       // ---- this warp's sums of the unit
-      const int i = u - u0, buf = i & 1;
-      if (i >= 2) ok = mbar_wait(red_empty(buf), uint32_t(i / 2 - 1) & 1u, abort_flag, kMoeWaitRedEmpty) && ok;
-      float4* red = reinterpret_cast<float4*>(smem + p.off_red) + (buf * kMoeConsumers + warp) * NT * 32 + lane;
+      const int i = u - u0, buf = i % RB;
+      if (i >= RB) ok = mbar_wait(red_empty(buf), uint32_t(i / RB - 1) & 1u, abort_flag, kMoeWaitRedEmpty) && ok;
+      float4* red = reinterpret_cast<float4*>(smem + p.off_red) + (buf * W + warp) * NT * 32 + lane;
 #pragma unroll
       for (int c = 0; c < NT; ++c) red[c * 32] = make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
       __syncwarp();
@@ -732,25 +760,21 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
     Place at = place0;
     for (int u = u0; u < u1; ++u, advance(at)) {
       const int chunk = at.chunk, seg = at.seg, tile = at.tile;
-      const int i = u - u0, buf = i & 1;
-      if (!mbar_wait(red_full(buf), uint32_t(i / 2) & 1u, abort_flag, kMoeWaitRedFull)) break;
-      const int count = route.chunk_count[chunk], first = route.chunk_first[chunk];
+      const int i = u - u0, buf = i % RB;
+      if (!mbar_wait(red_full(buf), uint32_t(i / RB) & 1u, abort_flag, kMoeWaitRedFull)) break;
+      const int count = route.chunk_count[chunk];
+      const short* pairs = route.list + route.chunk_first[chunk];
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
-        if (c > 0 && c * 8 >= count) break;
-        const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + (buf * kMoeConsumers * NT + c) * 32 + lane;
+        if (c > 0 && c * 8 >= (p.resident ? p.cols : count)) break;
+        const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + (buf * W * NT + c) * 32 + lane;
         float4 v = red[0];
 #pragma unroll
-        for (int w = 1; w < kMoeConsumers; ++w) {
+        for (int w = 1; w < W; ++w) {
           const float4 a = red[w * NT * 32];
           v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {  // columns 2 t4 and 2 t4 + 1
-          const int tok = c * 8 + 2 * t4 + k;
-          if (tok >= count) continue;
-          const int pair = route.list[first + tok];
-          const float a = k ? v.y : v.x, b = k ? v.w : v.z;
+        auto store = [&](int pair, float a, float b) {  // row g of either half
           if constexpr (GATE) {
             p.h[int64_t(pair) * p.I + tile * 8 + g] = a / (1.f + expf(-a)) * b;
           } else {
@@ -758,6 +782,17 @@ __global__ void __launch_bounds__(kMoeThreads, Cfg::NT == 1 ? 2 : 1) moe_kernel(
             z[0] = a;
             z[8] = b;
           }
+        };
+        // this lane has columns c 8 + 2 t4 and the next
+        if (p.resident) {
+          for (int k = 0; k < count; ++k) {
+            const int col = (GATE ? pairs[k] / p.top_k : pairs[k]) - c * 8;
+            if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);
+          }
+        } else {
+          const int col = c * 8 + 2 * t4;
+          if (col < count) store(pairs[col], v.x, v.z);
+          if (col + 1 < count) store(pairs[col + 1], v.y, v.w);
         }
       }
       __syncwarp();

@@ -122,6 +122,12 @@ def test_ids_outside_and_repeated(fmt):
     y = bf.moe_experts(x, ids, p, *layer.args)
     _check(y, x, ids, p, layer)
     assert (y[2] == 0).all()
+    for t in range(6):  # one token alone, its expert perhaps three times
+        _check(bf.moe_experts(x[t:t + 1], ids[t:t + 1], p[t:t + 1], *layer.args), x[t:t + 1], ids[t:t + 1], p[t:t + 1], layer)
+    many = torch.full((1, 16), 3, dtype=torch.int32, device=DEV)
+    layer16 = Layer(fmt, 16, 160, 96, seed=10)
+    p16 = torch.rand(1, 16, device=DEV, generator=_gen(3))
+    _check(bf.moe_experts(x[:1], many, p16, *layer16.args), x[:1], many, p16, layer16)
     none = torch.full((6, 3), -1, dtype=torch.int32, device=DEV)
     torch.empty(1 << 20, device=DEV).fill_(torch.nan)  # what the allocator hands out next
     y = bf.moe_experts(x, none, p, *layer.args)
