@@ -87,7 +87,6 @@ int launch_mx_gemm(MxGemmParams& gp, const bfp8_mxfp4_gemm_problem& p, int dev, 
 
 constexpr int kMoeMaxHidden = 8192;
 constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
-constexpr int kMoeMinStages = 3;
 constexpr int kMoeHalfSmem = 113 * 1024;
 
 int round_up(int x, int m) { return cdiv(x, m) * m; }
@@ -95,31 +94,39 @@ int round_up(int x, int m) { return cdiv(x, m) * m; }
 // How one kernel's units (segments of seg_len values of K) and shared memory
 // are laid out.
 struct MoeLayout {
-  int segments, seg_len, box, stages, smem, cols, resident;
+  int segments, seg_len, box, unit_stages, stages, smem, cols, resident;
   uint32_t off_b, off_ts, off_red, off_route, off_bars;
 };
 
 // K of `k` values in `segments` ranges, `entries` tokens or pairs that could
-// have a column of their own, within `limit` bytes of shared memory.
-bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int nt, int warps, int limit, int min_stages,
+// have a column of their own, within `limit` bytes of shared memory and with
+// min_slots stages for each consumer group.
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int nt, int warps, int limit, int min_slots,
                 MoeLayout* out) {
   const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
   const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, 8);
   out->box = cdiv(columns, unit_stages);
+  out->unit_stages = unit_stages;
   out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
   out->segments = cdiv(k, out->seg_len);
   out->resident = entries <= 8 * nt;
   out->cols = out->resident ? entries : std::min(P, 8 * nt);
   const int blocks = cdiv(std::min(k, out->seg_len), 128);
   const int stage = round_up(out->box * (2048 + (p.format ? 512 : 0)), 1024);
+  const int red_bufs = warps * nt >= 32 ? 1 : 2;
   const int b = blocks * 256 * out->cols, ts = round_up(blocks * 8 * nt * 4, 16);
-  const int red = (warps * nt >= 32 ? 1 : 2) * warps * nt * 512, route = round_up(moe_route_bytes(P), 16);
+  const int red = red_bufs * warps * nt * 512, route = round_up(moe_route_bytes(P), 16);
   const int scratch = P > 32 ? p.E * (cdiv(P, 32) + 1) * 4 : 0;
-  auto end_of = [&](int stages) { return 8 * (2 * stages + 4) + 16; };
-  const int stages = std::min(16, (limit - (1024 + b + ts + red + route + end_of(16))) / stage);
-  if (stages < min_stages || stages * stage < scratch) return false;
+  auto end_of = [&](int stages) { return 8 * (2 * stages + 2 * warps / moe_group_warps(warps, nt) * red_bufs) + 16 + 4 * stages; };
+  const int fixed = 1024 + b + ts + red + route + end_of(16);
+  const int groups = warps / moe_group_warps(warps, nt);
+  const int stages = std::min(16, (limit - fixed) / stage) / groups * groups;
+  if (stages < min_slots * groups) return false;
+  // the routing scratch lies where the ring and, unless they come first, the activations do
+  const int ring = std::max(stages * stage, round_up(scratch - (out->resident ? 0 : b), 128));
+  if (fixed + ring > limit) return false;
   out->stages = stages;
-  out->off_b = uint32_t(stages * stage);
+  out->off_b = uint32_t(ring);
   out->off_ts = out->off_b + uint32_t(b);
   out->off_red = out->off_ts + uint32_t(ts);
   out->off_route = out->off_red + uint32_t(red);
@@ -135,24 +142,25 @@ struct MoeShape {
 
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
   const int P = p.T * p.top_k, segments = cdiv(p.I, kMoeSegment);
-  auto fits = [&](int nt, int warps, int limit, int min_stages) {
+  auto fits = [&](int nt, int warps, int limit, int min_slots) {
     s->nt = nt;
     s->warps = warps;
-    return moe_layout(p, p.H, 1, p.T, nt, warps, limit, min_stages, &s->gate) &&
-           moe_layout(p, p.I, segments, P, nt, warps, limit, min_stages, &s->down);
+    return moe_layout(p, p.H, 1, p.T, nt, warps, limit, min_slots, &s->gate) &&
+           moe_layout(p, p.I, segments, P, nt, warps, limit, min_slots, &s->down);
   };
   // Up to 8 tokens: both kernels in half an SM's shared memory, so that DOWN
   // starts beside GATE and requests its weights while GATE runs.
-  if (p.T <= 8 && fits(1, 8, kMoeHalfSmem, 4)) return true;
+  if (p.T <= 8 && fits(1, 8, kMoeHalfSmem, 2)) return true;
   // Chunks of 16 where experts have more than four tokens on average, else of
   // 8: a ring twice as deep, and few experts are read twice.
-  if (p.T > 8 && P > 4 * p.E && fits(2, 16, kMaxSmem, kMoeMinStages)) return true;
-  return fits(1, 16, kMaxSmem, kMoeMinStages);
+  if (p.T > 8 && P > 4 * p.E && fits(2, 16, kMaxSmem, 2)) return true;
+  return fits(1, 16, kMaxSmem, 2) || fits(1, 8, kMaxSmem, 2) || fits(1, 8, kMaxSmem, 1);
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
+// A unit takes 8 rows and the 8 rows `half` further on.
 int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int64_t w_expert, int64_t w_row,
-             const void* scales, int E, int rows, int k) {
+             const void* scales, int E, int rows, int half, int k) {
   const uint64_t bytes = uint64_t(format ? k / 2 : k), full = bytes / 128;
   mp.columns = int(full);
   mp.rows = rows;
@@ -161,7 +169,7 @@ int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int
   if (!fn) return fail(BFP8_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
   auto encode = [&](CUtensorMap* map, const void* base, int rank, const cuuint64_t* dims, const cuuint64_t* strides,
                     const cuuint32_t* box, CUtensorMapSwizzle swizzle) {
-    const cuuint32_t ones[4] = {1, 1, 1, 1};
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
     CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank), const_cast<void*>(base), dims, strides, box, ones,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -172,11 +180,11 @@ int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int
   // stack follows in memory.
   mp.tail_reads_on = bytes % 128 != 0 && w_expert >= w_row * rows;
   const uint64_t columns = full + (mp.tail_reads_on ? 1 : 0);
-  if (columns > 0) {  // [128 bytes][rows][columns][experts]
-    const cuuint64_t dims[4] = {128, cuuint64_t(rows), columns, cuuint64_t(E)};
-    const cuuint64_t strides[3] = {cuuint64_t(w_row), 128, cuuint64_t(w_expert)};
-    const cuuint32_t box[4] = {128, 8, cuuint32_t(lay.box), 1};
-    if (int r = encode(&mp.map_w, w, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return r;
+  if (columns > 0) {  // [128 bytes][rows][columns][halves][experts]
+    const cuuint64_t dims[5] = {128, cuuint64_t(rows - half), columns, 2, cuuint64_t(E)};
+    const cuuint64_t strides[4] = {cuuint64_t(w_row), 128, cuuint64_t(w_row) * half, cuuint64_t(w_expert)};
+    const cuuint32_t box[5] = {128, 8, cuuint32_t(lay.box), 2, 1};
+    if (int r = encode(&mp.map_w, w, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return r;
   }
   if (bytes % 128) {
     const cuuint64_t dims[3] = {bytes, cuuint64_t(rows), cuuint64_t(E)};
@@ -187,11 +195,13 @@ int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int
   mp.rb = cdiv(rows, 128);
   mp.kb = cdiv(k, 128);
   mp.ws = scales;
-  if (format) {  // [512 bytes of a tile][K blocks][row tiles][experts]
-    const cuuint64_t dims[4] = {512, cuuint64_t(mp.kb), cuuint64_t(mp.rb), cuuint64_t(E)};
-    const cuuint64_t strides[3] = {512, cuuint64_t(mp.kb) * 512, cuuint64_t(mp.rb) * mp.kb * 512};
-    const cuuint32_t box[4] = {128, cuuint32_t(2 * lay.box), 1, 1};
-    if (int r = encode(&mp.map_s, scales, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return r;
+  if (format) {  // [512 bytes of a tile][K blocks][row tiles][halves][experts]
+    mp.scales_together = half == 8 || half % 128 == 0;
+    const uint64_t tiles = uint64_t(mp.kb) * 512;  // bytes of a row of tiles
+    const cuuint64_t dims[5] = {512, cuuint64_t(mp.kb), cuuint64_t(mp.rb), mp.scales_together ? 2u : 1u, cuuint64_t(E)};
+    const cuuint64_t strides[4] = {512, tiles, half == 8 ? 128 : std::max(1, half / 128) * tiles, tiles * mp.rb};
+    const cuuint32_t box[5] = {128, cuuint32_t(2 * lay.box), 1, mp.scales_together ? 2u : 1u, 1};
+    if (int r = encode(&mp.map_s, scales, 5, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE)) return r;
   }
   return BFP8_OK;
 }
@@ -229,6 +239,7 @@ int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms,
   mp.seg_len = lay.seg_len;
   mp.stages = lay.stages;
   mp.box = lay.box;
+  mp.unit_stages = lay.unit_stages;
   mp.off_b = lay.off_b;
   mp.off_ts = lay.off_ts;
   mp.off_red = lay.off_red;
@@ -388,9 +399,9 @@ int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
   mp.E = p.E;
   mp.top_k = p.top_k;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (int r = moe_maps(mp, s.gate, p.format, p.w13, p.w13_expert, p.w13_row, p.s13, p.E, 2 * p.I, p.H)) return r;
+  if (int r = moe_maps(mp, s.gate, p.format, p.w13, p.w13_expert, p.w13_row, p.s13, p.E, 2 * p.I, p.I, p.H)) return r;
   if (int r = launch_moe_any<true>(mp, s.gate, p.format, s, p.x_type, dev, num_sms, st)) return r;
-  if (int r = moe_maps(mp, s.down, p.format, p.w2, p.w2_expert, p.w2_row, p.s2, p.E, p.H, p.I)) return r;
+  if (int r = moe_maps(mp, s.down, p.format, p.w2, p.w2_expert, p.w2_row, p.s2, p.E, p.H, 8, p.I)) return r;
   if (int r = launch_moe_any<false>(mp, s.down, p.format, s, p.x_type, dev, num_sms, st)) return r;
   const MoeSumParams sp{mp.z, mp.routed, p.y, p.ldy, p.T, p.H, p.top_k, s.down.segments};
   cudaLaunchConfig_t cfg{};

@@ -18,13 +18,13 @@
 //   16 rows keep the last wave short (one token, 8 experts of I = 768: 768
 //   units over 148 CTAs) and need no sums across CTAs.
 // - A ring of shared-memory stages, 16 rows x up to 1 KB each; it runs across
-//   units, so the memory system sees one stream per SM.  Each half of a stage
-//   (8 rows) is one 4-D TMA box [128 bytes, 8 rows, up to 8 columns of 128
-//   bytes, 1 expert] in the 128-byte swizzle, which ldmatrix reads without
-//   conflicts.  (One bulk copy per row took the issuing warp about 60 clocks
-//   each, 1,000 a stage: more than the 700 that HBM takes to deliver it.)
-// - Consumer warps (8 or 16) in groups of four take stages in turn, and the
-//   128-wide K blocks of a stage in turn inside a group:
+//   units, so the memory system sees one stream per SM.  A stage is one 5-D TMA
+//   box [128 bytes, 8 rows, up to 8 columns of 128 bytes, 2 halves, 1 expert]
+//   in the 128-byte swizzle, which ldmatrix reads without conflicts.  (One
+//   bulk copy per row took the issuing warp about 60 clocks each, 1,000 a
+//   stage: more than the 700 that HBM takes to deliver it.)
+// - Consumer warps (8 or 16) work in groups, each with a unit and a ring of its
+//   own, and take the 128-wide K blocks of a stage in turn inside a group:
 //   ldmatrix, codes to f16 (exact: cvt, 128 codes per clock and SM), mma.sync
 //   m16n8k16 with fp32 accumulation, then the block's scales in fp32.  The
 //   legacy MMA is no bound here (one 8-token MMA per 256 weights is 0.09 of
@@ -40,7 +40,7 @@
 //   add them makes the slowest CTA do nearly all of it: 2.4 times the median
 //   CTA's time at 64 tokens.)  No result depends on the order of arrival.
 //
-// Warps: consumers, then the producer, then the finisher.
+// Warps: consumers, then one or two producers, then the finisher.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -58,7 +58,6 @@ namespace bfp8 {
 constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxExperts = 512;
-constexpr int kMoeGroupWarps = 4;  // consumer warps of a group; groups take stages in turn
 
 struct MoeParams {
   const void* x;  // [T, H] bf16 or fp16
@@ -70,11 +69,13 @@ struct MoeParams {
   const int* ids;
   const float* weights;
   int renormalize;
-  // This kernel's weights, rows of `columns` full 128-byte columns (map_w: 8
-  // rows x box columns) and perhaps one shorter (map_tail: 8 rows x 128 bytes).
+  // This kernel's weights, rows of `columns` full 128-byte columns (map_w: box
+  // columns of 8 rows and of the 8 rows of the unit's other half) and perhaps
+  // one shorter (map_tail: 128 bytes of 8 rows).
   CUtensorMap map_w, map_tail;
   int columns, rows, tail_reads_on;
-  CUtensorMap map_s;  // MXFP4: scale tiles, [128 bytes = 8 rows] x 2 box K blocks
+  CUtensorMap map_s;    // MXFP4: scale tiles, [128 bytes = 8 rows] x 2 box K blocks,
+  int scales_together;  // of both halves at once where they are a fixed distance apart
   const void* ws;     // block FP8: scales fp32 [E, rb, kb]
   int rb, kb;
   float* h;       // [T top_k, I]
@@ -83,6 +84,7 @@ struct MoeParams {
   int T, H, I, E, top_k;
   int segments, seg_len;  // K ranges of DOWN
   int stages, box;        // ring: stages, 128-byte columns of a stage
+  int unit_stages;        // stages of a unit
   int cols;               // token columns held
   int resident;           // every token (GATE) or pair (DOWN) has its own
   uint32_t off_b, off_ts, off_red, off_route, off_bars;  // shared memory
@@ -379,13 +381,19 @@ __global__ void __launch_bounds__(kMoeSumThreads) moe_sum_kernel(const MoeSumPar
   *reinterpret_cast<uint2*>(static_cast<T*>(p.y) + int64_t(t) * p.ldy + col) = out;
 }
 
+// Consumer warps work in groups, each on a unit of its own.  16 tokens a chunk
+// leave little room for rings: two groups of eight then.
+constexpr int moe_group_warps(int warps, int nt) { return nt == 2 ? warps / 2 : 4; }
+
 template <bool GATE_, bool MX_, int NT_, int WARPS_, class T_>
 struct MoeCfg {
   static constexpr bool GATE = GATE_, MX = MX_;
   static constexpr int NT = NT_;        // 8-token MMA tiles of a chunk
   static constexpr int WARPS = WARPS_;  // consumers
-  static constexpr int GROUPS = WARPS / kMoeGroupWarps;
-  static constexpr int THREADS = 32 * (WARPS + 2);
+  static constexpr int GROUP_WARPS = moe_group_warps(WARPS, NT);
+  static constexpr int GROUPS = WARPS / GROUP_WARPS;
+  static constexpr int PRODUCERS = WARPS == 16 ? 2 : 1;
+  static constexpr int THREADS = 32 * (WARPS + PRODUCERS + 1);
   static constexpr int RED_BUFS = WARPS * NT >= 32 ? 1 : 2;  // buffers of the warps' sums (512 NT bytes a warp)
   static constexpr int CTAS_PER_SM = WARPS == 8 ? 2 : 1;
   using T = T_;                   // x and y
@@ -470,8 +478,8 @@ __device__ __forceinline__ void moe_block(float (&acc)[Cfg::NT][4], uint32_t a_r
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(const __grid_constant__ MoeParams p) {
   constexpr bool GATE = Cfg::GATE, MX = Cfg::MX;
-  constexpr int NT = Cfg::NT, BB = Cfg::BLOCK_BYTES, W = Cfg::WARPS, RB = Cfg::RED_BUFS;
-  constexpr int THREADS = Cfg::THREADS;
+  constexpr int NT = Cfg::NT, BB = Cfg::BLOCK_BYTES, W = Cfg::WARPS, G = Cfg::GROUPS, RB = Cfg::RED_BUFS;
+  constexpr int THREADS = Cfg::THREADS, PRODUCERS = Cfg::PRODUCERS;
   using T = typename Cfg::T;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -480,25 +488,28 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   const int S = p.stages;
   // a stage: [half][column][8 rows][128 bytes], MXFP4: then [half][K block][8 rows][16 bytes] of scales
   const uint32_t half_bytes = uint32_t(p.box) * 1024u;
-  const uint32_t scale_copy = MX ? uint32_t(p.box) * 256u : 0u;  // of a half; stages stay 1024-byte aligned
-  const uint32_t scale_bytes = (scale_copy + 511u) & ~511u;
-  const uint32_t stage_bytes = 2u * (half_bytes + scale_bytes);
+  const uint32_t scale_copy = MX ? uint32_t(p.box) * 256u : 0u;  // of a half
+  const uint32_t stage_bytes = (2u * (half_bytes + scale_copy) + 1023u) & ~1023u;
   auto full = [&](int s) { return base + p.off_bars + 8u * uint32_t(s); };
   auto empty = [&](int s) { return base + p.off_bars + 8u * uint32_t(S + s); };
-  auto red_full = [&](int b) { return base + p.off_bars + 8u * uint32_t(2 * S + b); };
-  auto red_empty = [&](int b) { return base + p.off_bars + 8u * uint32_t(2 * S + 2 + b); };
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + p.off_bars + 8 * (2 * S + 4));
+  // of a group's buffer b
+  auto red_full = [&](int g, int b) { return base + p.off_bars + 8u * uint32_t(2 * S + g * RB + b); };
+  auto red_empty = [&](int g, int b) { return base + p.off_bars + 8u * uint32_t(2 * S + (G + g) * RB + b); };
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + p.off_bars + 8 * (2 * S + 2 * G * RB));
+  volatile int* issued = abort_flag + 4;  // [S] passes of each slot whose copies went out
   const MoeRoute route = moe_route_at(smem + p.off_route, p.T * p.top_k);
 
   if (tid == 0) {
     for (int s = 0; s < S; ++s) {
+      issued[s] = 0;
       mbar_init(full(s), 1u);
-      mbar_init(empty(s), kMoeGroupWarps);
+      mbar_init(empty(s), Cfg::GROUP_WARPS);
     }
-    for (int b = 0; b < 2; ++b) {
-      mbar_init(red_full(b), W);
-      mbar_init(red_empty(b), 1u);
-    }
+    for (int g = 0; g < G; ++g)
+      for (int b = 0; b < RB; ++b) {
+        mbar_init(red_full(g, b), Cfg::GROUP_WARPS);
+        mbar_init(red_empty(g, b), 1u);
+      }
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -567,66 +578,92 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   const int K = GATE ? p.H : p.I;
   const int64_t units = int64_t(chunks) * per_chunk;
   const int u0 = int(units * blockIdx.x / gridDim.x), u1 = int(units * (blockIdx.x + 1) / gridDim.x);
-  // A unit's place: chunk, K range, rows.
-  struct Place {
-    int chunk, seg, tile;
+  // The walk over this CTA's units, a row of up to G of them (one a group) with
+  // the same chunk and K range at a time.
+  struct Walk {
+    int u, chunk, seg, tile, count;  // first unit, its place, units of the row
   };
-  const Place place0 = {u0 / per_chunk, u0 % per_chunk / tiles, u0 % per_chunk % tiles};
-  auto advance = [&](Place& at) {
-    if (++at.tile == tiles) {
-      at.tile = 0;
-      if (++at.seg == p.segments) at.seg = 0, ++at.chunk;
+  auto begin = [&]() {
+    Walk w = {u0, u0 / per_chunk, u0 % per_chunk / tiles, u0 % per_chunk % tiles, 0};
+    w.count = min(G, min(u1 - w.u, tiles - w.tile));
+    return w;
+  };
+  auto next = [&](Walk& w) {
+    w.u += w.count;
+    w.tile += w.count;
+    if (w.tile == tiles) {
+      w.tile = 0;
+      if (++w.seg == p.segments) w.seg = 0, ++w.chunk;
     }
+    w.count = min(G, min(u1 - w.u, tiles - w.tile));
   };
+  // Every group has a ring of S / G slots of its own.  (In one ring for all, a
+  // slot would change groups from pass to pass, and a group ahead of another
+  // could take the parity of the pass before last for its own.)
+  const int ring = S / G, unit_stages = p.unit_stages;
   const int stage_blocks = p.box * (128 / BB);  // 128-wide K blocks of a stage
 
-  if (warp == W) {
+  if (warp >= W && warp < W + PRODUCERS) {
     // ---------------------------------------------------------------- producer
+    // One lane issues, for every PRODUCERS-th group: a stage costs it several
+    // hundred clocks of waits, addresses and the copy itself, and HBM delivers
+    // one in 700.
     if (lane == 0) {
       const uint64_t policy = policy_evict_first(), scale_policy = policy_evict_normal();
-      int n = 0, s = 0;
-      uint32_t phase = 1u;
       bool ok = true;
-      Place at = place0;
-      for (int u = u0; u < u1 && ok; ++u, advance(at)) {
-        const int expert = route.chunk_expert[at.chunk];
-        const int row[2] = {GATE ? at.tile * 8 : at.tile * 16, GATE ? p.I + at.tile * 8 : at.tile * 16 + 8};
-        const int first = at.seg * (p.seg_len / 128) * BB / 128;  // 128-byte columns
-        const int last = first + (min(p.seg_len, K - at.seg * p.seg_len) * BB / 128 + 127) / 128;
-        for (int c = first; c < last; c += p.box, ++n) {
-          if (n >= S && !(ok = mbar_wait(empty(s), phase, abort_flag, kMoeWaitEmpty))) break;
-          const uint32_t to = base + uint32_t(s) * stage_bytes;
+      int slot[G / PRODUCERS] = {};
+      uint32_t pass[G / PRODUCERS] = {};
+      for (Walk w = begin(); w.u < u1 && ok; next(w)) {
+        const int expert = route.chunk_expert[w.chunk];
+        const int first = w.seg * (p.seg_len / 128) * BB / 128;  // 128-byte columns
+        const int last = first + (min(p.seg_len, K - w.seg * p.seg_len) * BB / 128 + 127) / 128;
+        for (int i = 0, c = first; i < unit_stages && ok; ++i, c += p.box) {
           const int end = min(c + p.box, last);
-          // A short last column is read past the row's end, into the next
-          // row: consumers stop at K.  Behind the stack's last row there may
-          // be nothing to read.
-          if (end <= p.columns || (p.tail_reads_on && (expert < p.E - 1 || max(row[0], row[1]) + 8 < p.rows))) {
-            mbar_arrive_expect_tx(full(s), 2u * (half_bytes + scale_copy));
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              tma_load_4d(to + uint32_t(h) * half_bytes, &p.map_w, 0, row[h], c, expert, full(s), policy);
-          } else {  // column by column, zeros past the row
-            mbar_arrive_expect_tx(full(s), uint32_t(end - c) * 2048u + 2u * scale_copy);
-            for (int h = 0; h < 2; ++h)
-              for (int i = c; i < end; ++i)
-                tma_load_3d(to + uint32_t(h) * half_bytes + uint32_t(i - c) * 1024u, &p.map_tail, i * 128, row[h], expert,
-                            full(s), policy);
+          for (int k = 0; k < G / PRODUCERS; ++k) {
+            const int g = warp - W + k * PRODUCERS;
+            if (g >= w.count) break;
+            const int s = g * ring + slot[k];
+            if (pass[k] > 0 && !(ok = mbar_wait(empty(s), (pass[k] - 1) & 1u, abort_flag, kMoeWaitEmpty))) break;
+            issued[s] = int(pass[k]) + 1;
+            if (++slot[k] == ring) slot[k] = 0, ++pass[k];
+            const int row = (w.tile + g) * (GATE ? 8 : 16), row_b = row + (GATE ? p.I : 8);
+            const uint32_t to = base + uint32_t(s) * stage_bytes;
+            if (end <= c) {  // a shorter last K range: nothing left
+              mbar_arrive(full(s));
+              continue;
+            }
+            // A short last column is read past the row's end, into the next
+            // row: consumers stop at K.  Behind the stack's last row there may
+            // be nothing to read.
+            if (end <= p.columns || (p.tail_reads_on && (expert < p.E - 1 || row_b + 8 < p.rows))) {
+              mbar_arrive_expect_tx(full(s), 2u * (half_bytes + scale_copy));
+              tma_load_5d(to, &p.map_w, 0, row, c, 0, expert, full(s), policy);
+            } else {  // column by column, zeros past the row
+              mbar_arrive_expect_tx(full(s), uint32_t(end - c) * 2048u + 2u * scale_copy);
+              for (int j = c; j < end; ++j) {
+                tma_load_3d(to + uint32_t(j - c) * 1024u, &p.map_tail, j * 128, row, expert, full(s), policy);
+                tma_load_3d(to + half_bytes + uint32_t(j - c) * 1024u, &p.map_tail, j * 128, row_b, expert, full(s), policy);
+              }
+            }
+            if constexpr (MX) {
+              // A K block's scale words of 8 rows are 128 contiguous bytes of
+              // its tile, each next to the words of the rows 32, 64 and 96
+              // further on: a fourth is used here, the rest by the units that
+              // follow (from L2).
+              tma_load_5d(to + 2u * half_bytes, &p.map_s, (row & 31) * 16, 2 * c, row >> 7, 0, expert, full(s), scale_policy);
+              if (!p.scales_together)
+                tma_load_5d(to + 2u * half_bytes + scale_copy, &p.map_s, (row_b & 31) * 16, 2 * c, row_b >> 7, 0, expert,
+                            full(s), scale_policy);
+            }
           }
-          if constexpr (MX) {
-            // A K block's scale words of 8 rows are 128 contiguous bytes of
-            // its tile, each next to the words of the rows 32, 64 and 96
-            // further on: a fourth is used here, the rest by the units that
-            // follow (from L2).
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-              tma_load_4d(to + 2u * half_bytes + uint32_t(h) * scale_bytes, &p.map_s, (row[h] & 31) * 16, 2 * c, row[h] >> 7,
-                          expert, full(s), scale_policy);
-          }
-          if (++s == S) s = 0, phase ^= 1u;
         }
       }
-      for (int k = n > S ? n - S : 0; k < n; ++k) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMoeWaitDrain);
     }
+    __syncwarp();
+    // Every copy issued lands before the CTA may exit (the consumers have
+    // waited for them all, unless a wait gave up).
+    if (lane < S && issued[lane] > 0) mbar_wait(full(lane), uint32_t(issued[lane] - 1) & 1u, nullptr, kMoeWaitDrain);
     __syncwarp();
   } else if (warp < W) {
     // ---------------------------------------------------------------- consumers
@@ -635,21 +672,21 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
 #pragma unroll
     for (int c = 0; c < NT; ++c) b_lane[c] = base + p.off_b + uint32_t(min(c * 8 + g, p.cols - 1) * 64 + t4 * 16);
     if constexpr (!GATE) griddep_wait();  // h
-    constexpr int kStep = kMoeGroupWarps;
+    constexpr int kStep = Cfg::GROUP_WARPS;
     const int group = warp / kStep, warp_in_group = warp % kStep;
     const uint32_t a_lane = ((lane >> 3) & 1) * half_bytes + (lane & 7) * 128u;
-    int have = -1, count = 0, s = 0, turn = 0;
+    int have = -1, count = 0, done = 0, slot = 0;
     uint32_t phase = 0u;
     bool ok = true;
     // Block FP8 scales: lane l holds those of K blocks l and l + 32 of the
     // unit's two 8-row halves, requested a unit ahead where they change.
     float sc[2][2] = {}, sc_next[2][2] = {};
-    auto load_scales = [&](const Place& at) {
-      const float* e = static_cast<const float*>(p.ws) + int64_t(route.chunk_expert[at.chunk]) * p.rb * p.kb;
-      const int kb = at.seg * (p.seg_len / 128);
+    auto load_scales = [&](int chunk, int seg, int tile) {
+      const float* e = static_cast<const float*>(p.ws) + int64_t(route.chunk_expert[chunk]) * p.rb * p.kb;
+      const int kb = seg * (p.seg_len / 128);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        const int r = GATE ? half * p.I + at.tile * 8 : at.tile * 16 + 8 * half;
+        const int r = GATE ? half * p.I + tile * 8 : tile * 16 + 8 * half;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           const int b = kb + lane + 32 * j;
@@ -657,20 +694,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         }
       }
     };
-    // Does a unit read the same block scales as the one before it?
-    auto same_scales = [&](const Place& at) {
-      return at.tile != 0 && (GATE ? (at.tile & 15) != 0 && ((p.I + at.tile * 8) & 127) != 0 : (at.tile & 7) != 0);
-    };
-    Place at = place0;
-    if (!MX && u0 < u1) load_scales(at);
-    for (int u = u0; u < u1; ++u) {
-      const int chunk = at.chunk, seg = at.seg, tile = at.tile;
-      advance(at);  // the next unit's
-      if constexpr (!MX) {
-#pragma unroll
-        for (int half = 0; half < 2; ++half) sc[half][0] = sc_next[half][0], sc[half][1] = sc_next[half][1];
-        if (u + 1 < u1 && !same_scales(at)) load_scales(at);
-      }
+    Walk w = begin();
+    if (!MX && w.u < u1 && group < w.count) load_scales(w.chunk, w.seg, w.tile + group);
+    for (; w.u < u1; next(w)) {
+      const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
       const int k_len = min(p.seg_len, K - seg * p.seg_len);
       const int blocks = (k_len + 127) / 128;
       const int key = p.resident ? seg : chunk * p.segments + seg;
@@ -687,16 +714,29 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         }
         have = key;
       }
+      if constexpr (!MX) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) sc[half][0] = sc_next[half][0], sc[half][1] = sc_next[half][1];
+        // the next row's unit of this group (if it has none, what is loaded is not used)
+        Walk v = w;
+        next(v);
+        if (v.u < u1) {
+          const int t = v.tile + min(group, v.count - 1);
+          const bool same = group < w.count && v.chunk == chunk && v.seg == seg &&
+                            (GATE ? t >> 4 == tile >> 4 && (p.I + t * 8) >> 7 == (p.I + tile * 8) >> 7 : t >> 3 == tile >> 3);
+          if (!same) load_scales(v.chunk, v.seg, t);
+        }
+      }
+      if (group >= w.count) continue;
       // MXFP4: the 32-row quarter of the rows' scale tiles
       const uint32_t word_a = uint32_t(((GATE ? tile * 8 : tile * 16) >> 5) & 3) * 4u;
-      const uint32_t word_b = scale_bytes + uint32_t(((GATE ? p.I + tile * 8 : tile * 16 + 8) >> 5) & 3) * 4u;
+      const uint32_t word_b = scale_copy + uint32_t(((GATE ? p.I + tile * 8 : tile * 16 + 8) >> 5) & 3) * 4u;
       float acc[NT][4];
 #pragma unroll
       for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-      for (int b0 = 0; b0 < blocks; b0 += stage_blocks) {
-        const bool mine = turn == group;
-        if (++turn == Cfg::GROUPS) turn = 0;
-        if (mine) {
+      for (int b0 = 0; b0 < unit_stages * stage_blocks; b0 += stage_blocks) {
+        {
+          const int s = group * ring + slot;
           ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
           const int nb = min(stage_blocks, blocks - b0);
           const uint32_t stage = base + uint32_t(s) * stage_bytes;
@@ -739,16 +779,17 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
           __syncwarp();
           if (lane == 0) mbar_arrive(empty(s));
         }
-        if (++s == S) s = 0, phase ^= 1u;
+        if (++slot == ring) slot = 0, phase ^= 1u;
       }
       // ---- this warp's sums of the unit
-      const int i = u - u0, buf = i % RB;
-      if (i >= RB) ok = mbar_wait(red_empty(buf), uint32_t(i / RB - 1) & 1u, abort_flag, kMoeWaitRedEmpty) && ok;
+      const int buf = done % RB;
+      if (done >= RB) ok = mbar_wait(red_empty(group, buf), uint32_t(done / RB - 1) & 1u, abort_flag, kMoeWaitRedEmpty) && ok;
+      ++done;
       float4* red = reinterpret_cast<float4*>(smem + p.off_red) + (buf * W + warp) * NT * 32 + lane;
 #pragma unroll
       for (int c = 0; c < NT; ++c) red[c * 32] = make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
       __syncwarp();
-      if (lane == 0) mbar_arrive(red_full(buf));
+      if (lane == 0) mbar_arrive(red_full(group, buf));
     }
   } else {
     // ---------------------------------------------------------------- finisher
@@ -757,21 +798,27 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
       griddep_wait();  // z
       griddep_launch_dependents();
     }
-    Place at = place0;
-    for (int u = u0; u < u1; ++u, advance(at)) {
-      const int chunk = at.chunk, seg = at.seg, tile = at.tile;
-      const int i = u - u0, buf = i % RB;
-      if (!mbar_wait(red_full(buf), uint32_t(i / RB) & 1u, abort_flag, kMoeWaitRedFull)) break;
+    uint32_t done[G] = {};
+    Walk w = begin();
+    bool ok = true;
+    for (; w.u < u1 && ok; next(w)) {
+#pragma unroll
+     for (int group = 0; group < G; ++group) {
+      if (group >= w.count) break;
+      const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
+      const int buf = int(done[group] % RB);
+      if (!(ok = mbar_wait(red_full(group, buf), done[group] / RB & 1u, abort_flag, kMoeWaitRedFull))) break;
+      ++done[group];
       const int count = route.chunk_count[chunk];
       const short* pairs = route.list + route.chunk_first[chunk];
 #pragma unroll
       for (int c = 0; c < NT; ++c) {
         if (c > 0 && c * 8 >= (p.resident ? p.cols : count)) break;
-        const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + (buf * W * NT + c) * 32 + lane;
+        const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + ((buf * W + group * Cfg::GROUP_WARPS) * NT + c) * 32 + lane;
         float4 v = red[0];
 #pragma unroll
-        for (int w = 1; w < W; ++w) {
-          const float4 a = red[w * NT * 32];
+        for (int j = 1; j < Cfg::GROUP_WARPS; ++j) {
+          const float4 a = red[j * NT * 32];
           v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
         }
         auto store = [&](int pair, float a, float b) {  // row g of either half
@@ -796,7 +843,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive(red_empty(buf));
+      if (lane == 0) mbar_arrive(red_empty(group, buf));
+     }
     }
   }
 }

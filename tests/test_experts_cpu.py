@@ -173,3 +173,18 @@ def test_c_abi_refuses_before_any_launch():
         assert lib.bfp8_moe_workspace_bytes(ctypes.byref(bad)) == _native.BFP8_EINVAL, field
         assert lib.bfp8_launch_moe(ctypes.byref(bad), 256, None) == _native.BFP8_EINVAL, field
     assert lib.bfp8_launch_moe(ctypes.byref(m), 8, None) == _native.BFP8_EINVAL  # workspace alignment
+
+
+@needs_native
+@pytest.mark.parametrize("fmt", [0, 1])
+def test_every_allowed_layer_has_a_layout(fmt):
+    """Shared memory holds some layout of every size that the checks let through."""
+    lib = _native.capi()
+    m = _native.MoeProblem(x=16, ldx=8192, x_type=1, logits=16, ld_logits=512, logits_type=0, format=fmt, w13=16,
+                           w13_expert=16, w13_row=1 << 20, s13=16, w2=16, w2_expert=16, w2_row=1 << 20, s2=16, y=16, ldy=8192)
+    for m.T in (1, 2, 7, 8, 9, 16, 17, 33, 64):
+        for m.H in (32, 96, 1024, 2880, 4096, 4128, 7168, 8160, 8192):
+            for m.I in (32, 128, 1408, 2880, 4096, 4128, 14336, 16384 + 32):
+                for m.E in (1, 4, 128, 512):
+                    for m.top_k in {1, min(8, m.E), min(16, m.E)}:
+                        assert lib.bfp8_moe_workspace_bytes(ctypes.byref(m)) > 0, (m.T, m.H, m.I, m.E, m.top_k)
