@@ -99,12 +99,12 @@ struct MoeLayout {
 };
 
 // K of `k` values in `segments` ranges, `entries` tokens or pairs that could
-// have a column of their own, within `limit` bytes of shared memory and with
-// min_slots stages for each consumer group.
-bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int nt, int warps, int limit, int min_slots,
+// have a column of their own, in stages of up to max_box 128-byte columns and
+// within `limit` bytes of shared memory.
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int nt, int warps, int max_box, int limit,
                 MoeLayout* out) {
   const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
-  const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, 8);
+  const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, max_box);
   out->box = cdiv(columns, unit_stages);
   out->unit_stages = unit_stages;
   out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
@@ -121,7 +121,7 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
   const int fixed = 1024 + b + ts + red + route + end_of(16);
   const int groups = warps / moe_group_warps(warps, nt);
   const int stages = std::min(16, (limit - fixed) / stage) / groups * groups;
-  if (stages < min_slots * groups) return false;
+  if (stages < 2 * groups) return false;
   // the routing scratch lies where the ring and, unless they come first, the activations do
   const int ring = std::max(stages * stage, round_up(scratch - (out->resident ? 0 : b), 128));
   if (fixed + ring > limit) return false;
@@ -142,19 +142,23 @@ struct MoeShape {
 
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
   const int P = p.T * p.top_k, segments = cdiv(p.I, kMoeSegment);
-  auto fits = [&](int nt, int warps, int limit, int min_slots) {
+  auto fits = [&](int nt, int warps, int limit) {
     s->nt = nt;
     s->warps = warps;
-    return moe_layout(p, p.H, 1, p.T, nt, warps, limit, min_slots, &s->gate) &&
-           moe_layout(p, p.I, segments, P, nt, warps, limit, min_slots, &s->down);
+    auto one = [&](int k, int ranges, int entries, MoeLayout* lay) {
+      for (int box = 8; box >= 1; box /= 2)
+        if (moe_layout(p, k, ranges, entries, nt, warps, box, limit, lay)) return true;
+      return false;
+    };
+    return one(p.H, 1, p.T, &s->gate) && one(p.I, segments, P, &s->down);
   };
   // Up to 8 tokens: both kernels in half an SM's shared memory, so that DOWN
   // starts beside GATE and requests its weights while GATE runs.
-  if (p.T <= 8 && fits(1, 8, kMoeHalfSmem, 2)) return true;
+  if (p.T <= 8 && fits(1, 8, kMoeHalfSmem)) return true;
   // Chunks of 16 where experts have more than four tokens on average, else of
   // 8: a ring twice as deep, and few experts are read twice.
-  if (p.T > 8 && P > 4 * p.E && fits(2, 16, kMaxSmem, 2)) return true;
-  return fits(1, 16, kMaxSmem, 2) || fits(1, 8, kMaxSmem, 2) || fits(1, 8, kMaxSmem, 1);
+  if (p.T > 8 && P > 4 * p.E && fits(2, 16, kMaxSmem)) return true;
+  return fits(1, 16, kMaxSmem);
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
