@@ -83,6 +83,41 @@ int launch_mx_gemm(MxGemmParams& gp, const bfp8_mxfp4_gemm_problem& p, int dev, 
   return BFP8_OK;
 }
 
+// 256 x 256 tiles by CTA pairs.
+int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaStream_t stream) {
+  static std::atomic<uint64_t> done{0};
+  if (int r = allow_smem(reinterpret_cast<const void*>(&mx_pair_kernel), MxPairCfg::SMEM_BYTES, dev, done)) return r;
+  MxPairParams gp;
+  std::memset(&gp, 0, sizeof(gp));
+  const uint64_t scale_row = uint64_t(cdiv(p.K, 128)) * 512;
+  const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8, i32 = CU_TENSOR_MAP_DATA_TYPE_INT32;
+  const auto sw128 = CU_TENSOR_MAP_SWIZZLE_128B, plain = CU_TENSOR_MAP_SWIZZLE_NONE;
+  int r = make_map(&gp.map_x, u8, p.a, uint64_t(p.K / 2), uint64_t(p.M), uint64_t(p.lda), 128, 128, sw128);
+  if (!r) r = make_map(&gp.map_w, u8, p.b, uint64_t(p.K / 2), uint64_t(p.N), uint64_t(p.ldb), 128, 128, sw128);
+  if (!r) r = make_map(&gp.map_sx, i32, p.sa, scale_row / 4, uint64_t(cdiv(p.M, 128)), scale_row, 256, 1, plain);
+  if (!r) r = make_map(&gp.map_sw, i32, p.sb, scale_row / 4, uint64_t(cdiv(p.N, 128)), scale_row, 256, 1, plain);
+  if (!r) r = make_map(&gp.map_c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.c, uint64_t(p.N), uint64_t(p.M), uint64_t(p.ldc) * 2, 64, 128, sw128);
+  if (r) return r;
+  gp.K = p.K;
+  gp.k_stages = cdiv(p.K, 256);
+  gp.m_tiles = cdiv(p.M, 256);
+  gp.n_tiles = cdiv(p.N, 256);
+  gp.early = p.weights_ready ? 1 : 0;
+  const int64_t tiles = int64_t(gp.m_tiles) * gp.n_tiles;
+  if (tiles > INT32_MAX / 8) return fail(BFP8_EINVAL, "too many tiles for one launch");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * unsigned(std::min<int64_t>(tiles, num_sms / 2)));
+  cfg.blockDim = dim3(MxPairCfg::THREADS);
+  cfg.dynamicSmemBytes = MxPairCfg::SMEM_BYTES;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  set_pdl(cfg, attr);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, mx_pair_kernel, gp);
+  if (e == cudaSuccess) e = cudaGetLastError();
+  if (e != cudaSuccess) return cuda_fail(e, "MXFP4 GEMM launch");
+  return BFP8_OK;
+}
+
 // ---- the expert layer ---------------------------------------------------------------
 
 constexpr int kMoeMaxHidden = 8192;
@@ -359,6 +394,8 @@ int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* pp, void* stream) {
   if (p.M <= 16) return launch_mx_gemm<MxCfg<16, 5>>(gp, p, dev, num_sms, s);
   if (p.M <= 32) return launch_mx_gemm<MxCfg<32, 5>>(gp, p, dev, num_sms, s);
   if (p.M <= 64) return launch_mx_gemm<MxCfg<64, 4>>(gp, p, dev, num_sms, s);
+  // Pairs once their tiles fill the GPU.
+  if (int64_t(cdiv(p.M, 256)) * cdiv(p.N, 256) >= num_sms / 2) return launch_mx_pair(p, dev, num_sms, s);
   return launch_mx_gemm<MxCfg<128, 3>>(gp, p, dev, num_sms, s);
 }
 

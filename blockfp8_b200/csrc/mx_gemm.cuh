@@ -52,6 +52,7 @@ enum MxWaitSite : uint32_t {
   kMxWaitFull = 34,
   kMxWaitDone = 35,
   kMxWaitDrain = 36,
+  kMxWaitAcc = 37,
 };
 
 template <int BN_, int STAGES_>
@@ -226,6 +227,242 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc<1>(tmem, Cfg::TMEM_COLS);
+  }
+}
+
+// ---- prompts: CTA pairs ------------------------------------------------------------
+//
+// A cluster of two CTAs computes 256 tokens x 256 weight rows with
+// cta_group::2 MMAs (M = 256, N = 256, K = 64): each CTA holds 128 token rows
+// and 128 of the weight rows, so a stage of K = 256 costs an SM 35 KB of
+// shared-memory fill for 512 clocks of MMA (70 B per clock; the L2 delivers
+// about 62 to every SM at once, which is this kernel's bound, ahead of the
+// tensor cores).  Token rows are the MMA rows: a thread of the epilogue holds
+// one row's consecutive columns.
+//
+// TMEM: 256 accumulator columns and two stages' scales (each CTA its token
+// rows', and all 256 weight rows').  There is no room for a second
+// accumulator, so the epilogue first empties it into registers as bf16 (eight
+// warps, about 500 clocks of a tile's 8,192 at K = 4096), frees it, and stores
+// while the next tile runs: through shared memory and TMA, 64 columns at a
+// time.  Persistent, one pair on two SMs; tiles go to the pairs in groups of
+// eight token tiles, so that concurrent tiles share operands in L2.
+//
+// Warps: 0 TMA producer, 1 MMA issuer (the leader's) and TMEM owner, 4-11
+// epilogue.
+struct MxPairParams {
+  CUtensorMap map_x, map_w;    // codes [rows, K / 2] bytes: [128 x 128] boxes, 128-byte swizzle
+  CUtensorMap map_sx, map_sw;  // scale tiles [row tiles, k_tiles * 512 bytes]: 1 x 1024 bytes
+  CUtensorMap map_c;           // C [M, N]: [128 x 64] boxes, 128-byte swizzle
+  int K, k_stages, m_tiles, n_tiles;  // tiles of 256
+  int early;
+};
+
+struct MxPairCfg {
+  static constexpr int STAGES = 5;
+  static constexpr int THREADS = 384;
+  static constexpr int TILE_BYTES = 128 * 128, S_BYTES = 1024;
+  static constexpr int STAGE_BYTES = 2 * TILE_BYTES + 3 * S_BYTES;  // tokens, weights, scales of both
+  static constexpr int OUT_BYTES = 2 * 128 * 128;                   // [column half][128 rows][64 bf16]
+  static constexpr int TMEM_COLS = 512;
+  // tiles stay 1024-byte aligned, scales behind all of them
+  static constexpr int OFF_SCALES = STAGES * 2 * TILE_BYTES;
+  static constexpr int OFF_OUT = OFF_SCALES + STAGES * 3 * S_BYTES;
+  static constexpr int OFF_BARS = OFF_OUT + OUT_BYTES;
+  static_assert(OFF_OUT % 1024 == 0, "alignment");
+  static constexpr int SMEM_BYTES = 1024 + OFF_BARS + (2 * STAGES + 3) * 8 + 16;
+};
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 1)
+    mx_pair_kernel(const __grid_constant__ MxPairParams p) {
+  using Cfg = MxPairCfg;
+  constexpr int S = Cfg::STAGES;
+  griddep_launch_dependents();
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (base - raw);
+  auto x_tile = [&](int s) { return base + uint32_t(s * 2 * Cfg::TILE_BYTES); };
+  auto w_tile = [&](int s) { return x_tile(s) + Cfg::TILE_BYTES; };
+  auto sx_tile = [&](int s) { return base + uint32_t(Cfg::OFF_SCALES + s * 3 * Cfg::S_BYTES); };
+  auto sw_tile = [&](int s, int h) { return sx_tile(s) + uint32_t((1 + h) * Cfg::S_BYTES); };
+  const uint32_t bars = base + Cfg::OFF_BARS;
+  auto full = [&](int s) { return bars + 8u * uint32_t(s); };  // the leader's: both CTAs' copies
+  auto empty = [&](int s) { return bars + 8u * uint32_t(S + s); };
+  const uint32_t acc_full = bars + 8u * uint32_t(2 * S), acc_empty = acc_full + 8u, done = acc_full + 16u;
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BARS + 8 * (2 * S + 3));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_rank();
+  const bool leader = rank == 0;
+  const int pair = int(blockIdx.x >> 1), pairs = int(gridDim.x >> 1);
+  const int tiles = p.m_tiles * p.n_tiles;
+  auto place = [&](int t, int& mt, int& nt) {  // groups of 8 token tiles, token tiles first
+    const int group = t / (8 * p.n_tiles), rest = t - group * 8 * p.n_tiles;
+    const int rows = min(8, p.m_tiles - group * 8);
+    nt = rest / rows;
+    mt = group * 8 + rest - nt * rows;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S; ++s) {
+      mbar_init(full(s), 1);
+      mbar_init(empty(s), 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_empty, 16);  // the eight epilogue warps of both CTAs
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    tma_prefetch_desc(&p.map_x);
+    tma_prefetch_desc(&p.map_w);
+    tma_prefetch_desc(&p.map_c);
+  }
+  if (warp == 1) {
+    tmem_alloc<2>(smem_u32(misc), Cfg::TMEM_COLS);
+    tmem_relinquish<2>();
+  }
+  tc_fence_before();
+  cluster_sync();  // the peer's barriers are initialised before any remote use
+  tc_fence_after();
+  const uint32_t tmem = misc[0];
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol = policy_evict_normal();
+      auto load_w = [&](int s, int k, int nt) {
+        const uint32_t bar = map_shared_rank(full(s), 0);
+        if (leader) mbar_arrive_expect_tx(full(s), 2u * Cfg::STAGE_BYTES);
+        tma_load_2d_pair(w_tile(s), &p.map_w, k * 128, nt * 256 + int(rank) * 128, bar, pol);
+        tma_load_2d_pair(sw_tile(s, 0), &p.map_sw, k * 256, nt * 2, bar, pol);
+        tma_load_2d_pair(sw_tile(s, 1), &p.map_sw, k * 256, nt * 2 + 1, bar, pol);
+      };
+      auto load_x = [&](int s, int k, int mt) {
+        const uint32_t bar = map_shared_rank(full(s), 0);
+        tma_load_2d_pair(x_tile(s), &p.map_x, k * 128, mt * 256 + int(rank) * 128, bar, pol);
+        tma_load_2d_pair(sx_tile(s), &p.map_sx, k * 256, mt * 2 + int(rank), bar, pol);
+      };
+      int pre = 0;
+      if (p.early && pair < tiles) {
+        int mt, nt;
+        place(pair, mt, nt);
+        for (; pre < S && pre < p.k_stages; ++pre) load_w(pre, pre, nt);
+      }
+      griddep_wait();
+      int i = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int mt, nt;
+        place(t, mt, nt);
+        for (int k = 0; k < p.k_stages; ++k, ++i) {
+          const int s = i % S;
+          if (i >= S && !(ok = mbar_wait(empty(s), uint32_t(i / S - 1) & 1u, abort_flag, kMxWaitEmpty))) break;
+          if (i >= pre) load_w(s, k, nt);
+          load_x(s, k, mt);
+        }
+      }
+      // The leader's MMAs read what was loaded last; every copy has landed once
+      // they are done.  (A CTA stays until its peer gets here, so that no
+      // commit arrives on a barrier that is gone.)
+      for (int k = i > S ? i - S : 0; k < i; ++k) {
+        if (ok) mbar_wait(empty(k % S), uint32_t(k / S) & 1u, abort_flag, kMxWaitDrain);
+        else if (leader) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMxWaitDrain);  // a wait gave up
+      }
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (leader && lane == 0) {
+      constexpr uint32_t idesc = idesc_mxf4(256, 256);
+      int i = 0, n = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+        if (n > 0 && !mbar_wait(acc_empty, uint32_t(n - 1) & 1u, abort_flag, kMxWaitAcc)) break;
+        tc_fence_after();
+        for (int k = 0; k < p.k_stages; ++k, ++i) {
+          const int s = i % S;
+          if (!(ok = mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull))) break;
+          tc_fence_after();
+          const int left = p.K - k * 256;
+          const int steps = left >= 256 ? 4 : (left + 63) / 64;
+          const uint32_t sf = tmem + 256u + uint32_t(32 * (i & 1));  // [kt][4 token, 8 weight columns, 4 unused]
+          for (int kt = 0; kt < (steps + 1) / 2; ++kt) {
+            tmem_cp_scales_pair(sf + uint32_t(16 * kt), smem_desc_scales(sx_tile(s) + uint32_t(512 * kt)));
+            tmem_cp_scales_pair(sf + uint32_t(16 * kt + 4), smem_desc_scales(sw_tile(s, 0) + uint32_t(512 * kt)));
+            tmem_cp_scales_pair(sf + uint32_t(16 * kt + 8), smem_desc_scales(sw_tile(s, 1) + uint32_t(512 * kt)));
+          }
+          const uint64_t a = smem_desc_k128_sw128(x_tile(s)), b = smem_desc_k128_sw128(w_tile(s));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (j < steps)
+              mma_mxf4<2>(tmem, a + 2 * j, b + 2 * j, idesc | idesc_scale_half(j & 1), sf + uint32_t(16 * (j >> 1)),
+                          sf + uint32_t(16 * (j >> 1) + 4), (k > 0 || j > 0) ? 1u : 0u);
+          mma_commit<2>(empty(s));
+          mma_commit<2>(map_shared_rank(empty(s), 1));
+        }
+        mma_commit<2>(acc_full);
+        mma_commit<2>(map_shared_rank(acc_full, 1));
+      }
+      mma_commit<2>(done);
+      mbar_wait(done, 0, nullptr, kMxWaitDone);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    griddep_wait();  // C
+    const int q = warp & 3, half = (warp - 4) >> 2;  // lanes 32 q .., columns 128 half ..
+    const int row = 32 * q + lane;
+    const uint32_t t_lane = tmem + (uint32_t(32 * q) << 16) + uint32_t(128 * half);
+    const uint32_t out = base + uint32_t(Cfg::OFF_OUT + half * 128 * 128);
+    const uint32_t empty_bar = map_shared_rank(acc_empty, 0);
+    int n = 0;
+    for (int t = pair; t < tiles; t += pairs, ++n) {
+      if (!mbar_wait(acc_full, uint32_t(n) & 1u, abort_flag, kMxWaitAcc)) break;
+      tc_fence_after();
+      uint32_t packed[64];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float v[32];
+        tmem_ld32(t_lane + uint32_t(32 * c), v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+          packed[c * 16 + j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(empty_bar);  // the next tile's MMAs may start
+      int mt, nt;
+      place(t, mt, nt);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {  // 64 columns: 128 bytes a row
+        // the store that read this buffer last is done
+        if ((warp & 3) == 0 && lane == 0) bulk_wait_read0();
+        named_bar_sync(1 + half, 128);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          st_shared_v4(out + uint32_t(row * 128 + ((j ^ (row & 7)) << 4)), packed[c * 32 + 4 * j], packed[c * 32 + 4 * j + 1],
+                       packed[c * 32 + 4 * j + 2], packed[c * 32 + 4 * j + 3]);
+        fence_proxy_async_smem();
+        named_bar_sync(1 + half, 128);
+        const int col = nt * 256 + half * 128 + c * 64;
+        if ((warp & 3) == 0 && lane == 0 && !*abort_flag) {
+          tma_store_2d(&p.map_c, col, mt * 256 + int(rank) * 128, out);
+          bulk_commit();
+        }
+      }
+    }
+    if ((warp & 3) == 0 && lane == 0) bulk_wait0();
+  }
+  tc_fence_before();
+  // The leader's MMAs and both CTAs' remote arrivals are over before either
+  // frees TMEM or exits.
+  cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc<2>(tmem, Cfg::TMEM_COLS);
   }
 }
 
