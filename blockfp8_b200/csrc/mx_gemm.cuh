@@ -15,11 +15,15 @@
 //
 // Stages of K = 256: 128 bytes of codes per row (one 128-byte-swizzled TMA
 // box for the weights, one for the tokens) and 512 bytes of scales per 128
-// rows per 128 of K (bulk copies; the scale layout is the order in which
-// tcgen05.cp wants them).  Per stage one thread issues the scale copies to
-// TMEM and four MMAs of K = 64; tcgen05 runs them in order.
+// rows per 128 of K (bulk copies).  The epilogue's warps, which have nothing
+// else to do in the loop, carry the scales on into TMEM: row r of a tile lies
+// in lane r % 32, column r / 32, the same in each warp's 32 lanes, and the
+// layout in memory is that order, so a warp needs one 16-byte load a lane and
+// tile.  (tcgen05.cp would do the same on the tensor pipe, where a copy of
+// 512 bytes costs about 170 clocks and does not overlap MMAs.)  One thread
+// issues four MMAs of K = 64 a stage.
 //
-// Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-5 epilogue.
+// Warps: 0 TMA producer, 1 MMA issuer and TMEM owner, 2-5 scales, epilogue.
 #pragma once
 
 #include <cuda.h>
@@ -53,6 +57,7 @@ enum MxWaitSite : uint32_t {
   kMxWaitDone = 35,
   kMxWaitDrain = 36,
   kMxWaitAcc = 37,
+  kMxWaitScales = 38,
 };
 
 template <int BN_, int STAGES_>
@@ -62,12 +67,12 @@ struct MxCfg {
   static constexpr int W_BYTES = 128 * 128, X_BYTES = BN * 128, S_BYTES = 1024;  // per stage
   static constexpr int STAGE_BYTES = W_BYTES + X_BYTES + 2 * S_BYTES;
   static constexpr int ACC_COLS = BN < 32 ? 32 : BN;
-  // two stages' scales: 2 K tiles x (4 weight + 4 token) columns each
-  static constexpr int TMEM_COLS = BN <= 32 ? 64 : (BN == 64 ? 128 : 256);
-  static_assert(ACC_COLS + 32 <= TMEM_COLS, "TMEM");
+  // behind the accumulator every stage's scales: 2 K tiles x (4 weight + 4 token) columns
+  static constexpr int TMEM_COLS = BN <= 64 ? 128 : 256;
+  static_assert(ACC_COLS + 16 * STAGES <= TMEM_COLS, "TMEM");
   static constexpr int RING = STAGES * STAGE_BYTES;
   static_assert(RING >= 128 * BN * 4, "the ring holds the tile's fp32 sums at the end");
-  static constexpr int SMEM_BYTES = 1024 + RING + (2 * STAGES + 1) * 8 + 16;
+  static constexpr int SMEM_BYTES = 1024 + RING + (3 * STAGES + 1) * 8 + 16;
 };
 
 template <class Cfg>
@@ -85,8 +90,9 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
   const uint32_t bars = base + Cfg::RING;
   auto full = [&](int s) { return bars + 8u * uint32_t(s); };
   auto empty = [&](int s) { return bars + 8u * uint32_t(S + s); };
-  const uint32_t done = bars + 8u * uint32_t(2 * S);
-  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::RING + 8 * (2 * S + 1));
+  auto scaled = [&](int s) { return bars + 8u * uint32_t(2 * S + s); };  // the stage's scales are in TMEM
+  const uint32_t done = bars + 8u * uint32_t(3 * S);
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::RING + 8 * (3 * S + 1));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -98,7 +104,7 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
   const int L = s1 - s0;
 
   if (warp == 0 && lane == 0) {
-    for (int i = 0; i < 2 * S + 1; ++i) mbar_init(bars + 8u * uint32_t(i), 1u);
+    for (int i = 0; i < 3 * S + 1; ++i) mbar_init(bars + 8u * uint32_t(i), i >= 2 * S && i < 3 * S ? 4u : 1u);
     *abort_flag = 0;
     fence_barrier_init();
     tma_prefetch_desc(&p.map_w);
@@ -153,14 +159,11 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
       for (int i = 0; i < L; ++i) {
         const int s = i % S;
         if (!mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull)) break;
+        if (!mbar_wait(scaled(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitScales)) break;
         tc_fence_after();
         const int left = p.K - (s0 + i) * 256;  // values of K from this stage on
         const int steps = left >= 256 ? 4 : (left + 63) / 64;
-        const uint32_t sf = scales + uint32_t(16 * (i & 1));  // [kt][4 weight + 4 token] columns
-        for (int kt = 0; kt < (steps + 1) / 2; ++kt) {
-          tmem_cp_scales(sf + uint32_t(8 * kt), smem_desc_scales(sw_tile(s) + uint32_t(512 * kt)));
-          tmem_cp_scales(sf + uint32_t(8 * kt + 4), smem_desc_scales(sx_tile(s) + uint32_t(512 * kt)));
-        }
+        const uint32_t sf = scales + uint32_t(16 * s);  // [kt][4 weight + 4 token] columns
         const uint64_t a = smem_desc_k128_sw128(w_tile(s)), b = smem_desc_k128_sw128(x_tile(s));
 #pragma unroll
         for (int k = 0; k < 4; ++k)  // K = 64 codes = 32 bytes = 2 descriptor units
@@ -173,6 +176,27 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
       mbar_wait(done, 0, nullptr, kMxWaitDone);
     }
     __syncwarp();
+  } else {
+    // Scales of stage i: its TMEM columns were last read by the MMAs whose end
+    // let the producer refill the stage.
+    const uint32_t t_lane = tmem + (uint32_t(32 * (warp & 3)) << 16) + uint32_t(Cfg::ACC_COLS);
+    for (int i = 0; i < L; ++i) {
+      const int s = i % S;
+      if (!mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull)) break;
+      uint32_t r[16];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const uint4 w = ld_shared_v4(sw_tile(s) + uint32_t(512 * kt + 16 * lane));
+        const uint4 x = ld_shared_v4(sx_tile(s) + uint32_t(512 * kt + 16 * lane));
+        r[8 * kt] = w.x, r[8 * kt + 1] = w.y, r[8 * kt + 2] = w.z, r[8 * kt + 3] = w.w;
+        r[8 * kt + 4] = x.x, r[8 * kt + 5] = x.y, r[8 * kt + 6] = x.z, r[8 * kt + 7] = x.w;
+      }
+      tmem_st16(t_lane + uint32_t(16 * s), r);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(scaled(s));
+    }
   }
   // Every load has landed and every MMA is done: the ring is free.
   tc_fence_before();
@@ -240,19 +264,20 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
 // tensor cores).  Token rows are the MMA rows: a thread of the epilogue holds
 // one row's consecutive columns.
 //
-// TMEM: 256 accumulator columns and two stages' scales (each CTA its token
-// rows', and all 256 weight rows').  There is no room for a second
-// accumulator, so the epilogue first empties it into registers as bf16 (eight
-// warps, about 500 clocks of a tile's 8,192 at K = 4096), frees it, and stores
-// while the next tile runs: through shared memory and TMA, 64 columns at a
-// time.  Persistent, one pair on two SMs; tiles go to the pairs in groups of
-// eight token tiles, so that concurrent tiles share operands in L2.
+// TMEM: 256 accumulator columns and every stage's scales (each CTA its token
+// rows', and all 256 weight rows').
+// There is no room for a second accumulator, so the epilogue first empties it
+// into registers as bf16 (eight warps, about 500 clocks of a tile's 8,192 at
+// K = 4096), frees it, and stores while the next tile runs: through shared
+// memory and TMA, 64 columns at a time.  Persistent, one pair on two SMs;
+// tiles go to the pairs in groups of eight token tiles, so that concurrent
+// tiles share operands in L2.
 //
-// Warps: 0 TMA producer, 1 MMA issuer (the leader's) and TMEM owner, 4-11
-// epilogue.
+// Warps: 0 TMA producer of codes, 2 of scales, 1 MMA issuer and TMEM owner, 3
+// issuer of the scales' copies into TMEM (1 and 3 the leader's), 4-11 epilogue.
 struct MxPairParams {
   CUtensorMap map_x, map_w;    // codes [rows, K / 2] bytes: [128 x 128] boxes, 128-byte swizzle
-  CUtensorMap map_sx, map_sw;  // scale tiles [row tiles, k_tiles * 512 bytes]: 1 x 1024 bytes
+  CUtensorMap map_sx, map_sw;  // scale tiles [row tiles, k_tiles * 512 bytes]: 1 and 2 x 1024 bytes
   CUtensorMap map_c;           // C [M, N]: [128 x 64] boxes, 128-byte swizzle
   int K, k_stages, m_tiles, n_tiles;  // tiles of 256
   int early;
@@ -262,7 +287,7 @@ struct MxPairCfg {
   static constexpr int STAGES = 5;
   static constexpr int THREADS = 384;
   static constexpr int TILE_BYTES = 128 * 128, S_BYTES = 1024;
-  static constexpr int STAGE_BYTES = 2 * TILE_BYTES + 3 * S_BYTES;  // tokens, weights, scales of both
+  static constexpr int SCALE_COLS = 24;  // of a stage: [K tile][4 token, 8 weight columns]
   static constexpr int OUT_BYTES = 2 * 128 * 128;                   // [column half][128 rows][64 bf16]
   static constexpr int TMEM_COLS = 512;
   // tiles stay 1024-byte aligned, scales behind all of them
@@ -270,7 +295,8 @@ struct MxPairCfg {
   static constexpr int OFF_OUT = OFF_SCALES + STAGES * 3 * S_BYTES;
   static constexpr int OFF_BARS = OFF_OUT + OUT_BYTES;
   static_assert(OFF_OUT % 1024 == 0, "alignment");
-  static constexpr int SMEM_BYTES = 1024 + OFF_BARS + (2 * STAGES + 3) * 8 + 16;
+  static constexpr int SMEM_BYTES = 1024 + OFF_BARS + (4 * STAGES + 4) * 8 + 16;
+  static_assert(256 + STAGES * SCALE_COLS <= TMEM_COLS, "TMEM");
 };
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 1)
@@ -285,12 +311,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
   auto x_tile = [&](int s) { return base + uint32_t(s * 2 * Cfg::TILE_BYTES); };
   auto w_tile = [&](int s) { return x_tile(s) + Cfg::TILE_BYTES; };
   auto sx_tile = [&](int s) { return base + uint32_t(Cfg::OFF_SCALES + s * 3 * Cfg::S_BYTES); };
-  auto sw_tile = [&](int s, int h) { return sx_tile(s) + uint32_t((1 + h) * Cfg::S_BYTES); };
   const uint32_t bars = base + Cfg::OFF_BARS;
   auto full = [&](int s) { return bars + 8u * uint32_t(s); };  // the leader's: both CTAs' copies
   auto empty = [&](int s) { return bars + 8u * uint32_t(S + s); };
-  const uint32_t acc_full = bars + 8u * uint32_t(2 * S), acc_empty = acc_full + 8u, done = acc_full + 16u;
-  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BARS + 8 * (2 * S + 3));
+  auto sfull = [&](int s) { return bars + 8u * uint32_t(2 * S + s); };   // the leader's: both CTAs' scales
+  auto scaled = [&](int s) { return bars + 8u * uint32_t(3 * S + s); };  // the leader's: they are in TMEM
+  const uint32_t leader_bars = map_shared_rank(bars, 0), peer_bars = map_shared_rank(bars, 1);
+  const uint32_t acc_full = bars + 8u * uint32_t(4 * S), acc_empty = acc_full + 8u, done = acc_full + 16u;
+  const uint32_t copied = acc_full + 24u;
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BARS + 8 * (4 * S + 4));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -309,10 +338,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
     for (int s = 0; s < S; ++s) {
       mbar_init(full(s), 1);
       mbar_init(empty(s), 1);
+      mbar_init(sfull(s), 1);
+      mbar_init(scaled(s), 1);
     }
     mbar_init(acc_full, 1);
     mbar_init(acc_empty, 16);  // the eight epilogue warps of both CTAs
     mbar_init(done, 1);
+    mbar_init(copied, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -334,16 +366,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
     if (lane == 0) {
       const uint64_t pol = policy_evict_normal();
       auto load_w = [&](int s, int k, int nt) {
-        const uint32_t bar = map_shared_rank(full(s), 0);
-        if (leader) mbar_arrive_expect_tx(full(s), 2u * Cfg::STAGE_BYTES);
-        tma_load_2d_pair(w_tile(s), &p.map_w, k * 128, nt * 256 + int(rank) * 128, bar, pol);
-        tma_load_2d_pair(sw_tile(s, 0), &p.map_sw, k * 256, nt * 2, bar, pol);
-        tma_load_2d_pair(sw_tile(s, 1), &p.map_sw, k * 256, nt * 2 + 1, bar, pol);
+        if (leader) mbar_arrive_expect_tx(full(s), 4u * Cfg::TILE_BYTES);
+        tma_load_2d_pair(w_tile(s), &p.map_w, k * 128, nt * 256 + int(rank) * 128, leader_bars + 8u * uint32_t(s), pol);
       };
       auto load_x = [&](int s, int k, int mt) {
-        const uint32_t bar = map_shared_rank(full(s), 0);
-        tma_load_2d_pair(x_tile(s), &p.map_x, k * 128, mt * 256 + int(rank) * 128, bar, pol);
-        tma_load_2d_pair(sx_tile(s), &p.map_sx, k * 256, mt * 2 + int(rank), bar, pol);
+        tma_load_2d_pair(x_tile(s), &p.map_x, k * 128, mt * 256 + int(rank) * 128, leader_bars + 8u * uint32_t(s), pol);
       };
       int pre = 0;
       if (p.early && pair < tiles) {
@@ -373,6 +400,54 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
       }
     }
     __syncwarp();
+  } else if (warp == 2) {
+    if (lane == 0) {
+      const uint64_t pol = policy_evict_normal();
+      griddep_wait();
+      int i = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        int mt, nt;
+        place(t, mt, nt);
+        for (int k = 0; k < p.k_stages; ++k, ++i) {
+          const int s = i % S;
+          if (i >= S && !(ok = mbar_wait(empty(s), uint32_t(i / S - 1) & 1u, abort_flag, kMxWaitEmpty))) break;
+          if (leader) mbar_arrive_expect_tx(sfull(s), 6u * Cfg::S_BYTES);
+          const uint32_t bar = leader_bars + 8u * uint32_t(2 * S + s);
+          tma_load_2d_pair(sx_tile(s), &p.map_sx, k * 256, mt * 2 + int(rank), bar, pol);
+          tma_load_2d_pair(sx_tile(s) + Cfg::S_BYTES, &p.map_sw, k * 256, nt * 2, bar, pol);
+        }
+      }
+      if (leader)
+        for (int k = i > S ? i - S : 0; k < i; ++k) mbar_wait(sfull(k % S), uint32_t(k / S) & 1u, nullptr, kMxWaitDrain);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // Scales into TMEM, by a thread of their own: issuing six copies takes one
+    // thread about 500 clocks a stage, as long as the MMAs run.  A stage's
+    // columns were last read by the MMAs whose end let it be refilled.
+    if (leader && lane == 0) {
+      int i = 0;
+      bool ok = true;
+      for (int t = pair; t < tiles && ok; t += pairs) {
+        for (int k = 0; k < p.k_stages; ++k, ++i) {
+          const int s = i % S;
+          if (!(ok = mbar_wait(sfull(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull))) break;
+          tc_fence_after();
+          const uint32_t sf = tmem + 256u + uint32_t(Cfg::SCALE_COLS * s);  // [kt][4 token, 8 weight columns]
+          const uint64_t desc = smem_desc_scales(sx_tile(s));
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int h = 0; h < 3; ++h)  // token rows, weight rows 0-127, 128-255
+              tmem_cp_scales_pair(sf + uint32_t(12 * kt + 4 * h), desc + uint64_t((h * Cfg::S_BYTES + 512 * kt) >> 4));
+          mma_commit<2>(scaled(s));
+        }
+      }
+      mma_commit<2>(copied);
+      mbar_wait(copied, 0, nullptr, kMxWaitDone);
+    }
+    __syncwarp();
   } else if (warp == 1) {
     if (leader && lane == 0) {
       constexpr uint32_t idesc = idesc_mxf4(256, 256);
@@ -380,30 +455,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs, ++n) {
         if (n > 0 && !mbar_wait(acc_empty, uint32_t(n - 1) & 1u, abort_flag, kMxWaitAcc)) break;
-        tc_fence_after();
         for (int k = 0; k < p.k_stages; ++k, ++i) {
           const int s = i % S;
           if (!(ok = mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull))) break;
+          if (!(ok = mbar_wait(scaled(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitScales))) break;
           tc_fence_after();
           const int left = p.K - k * 256;
           const int steps = left >= 256 ? 4 : (left + 63) / 64;
-          const uint32_t sf = tmem + 256u + uint32_t(32 * (i & 1));  // [kt][4 token, 8 weight columns, 4 unused]
-          for (int kt = 0; kt < (steps + 1) / 2; ++kt) {
-            tmem_cp_scales_pair(sf + uint32_t(16 * kt), smem_desc_scales(sx_tile(s) + uint32_t(512 * kt)));
-            tmem_cp_scales_pair(sf + uint32_t(16 * kt + 4), smem_desc_scales(sw_tile(s, 0) + uint32_t(512 * kt)));
-            tmem_cp_scales_pair(sf + uint32_t(16 * kt + 8), smem_desc_scales(sw_tile(s, 1) + uint32_t(512 * kt)));
-          }
+          const uint32_t sf = tmem + 256u + uint32_t(Cfg::SCALE_COLS * s);
           const uint64_t a = smem_desc_k128_sw128(x_tile(s)), b = smem_desc_k128_sw128(w_tile(s));
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             if (j < steps)
-              mma_mxf4<2>(tmem, a + 2 * j, b + 2 * j, idesc | idesc_scale_half(j & 1), sf + uint32_t(16 * (j >> 1)),
-                          sf + uint32_t(16 * (j >> 1) + 4), (k > 0 || j > 0) ? 1u : 0u);
+              mma_mxf4<2>(tmem, a + 2 * j, b + 2 * j, idesc | idesc_scale_half(j & 1), sf + uint32_t(12 * (j >> 1)),
+                          sf + uint32_t(12 * (j >> 1) + 4), (k > 0 || j > 0) ? 1u : 0u);
           mma_commit<2>(empty(s));
-          mma_commit<2>(map_shared_rank(empty(s), 1));
+          mma_commit<2>(peer_bars + 8u * uint32_t(S + s));
         }
         mma_commit<2>(acc_full);
-        mma_commit<2>(map_shared_rank(acc_full, 1));
+        mma_commit<2>(peer_bars + 8u * uint32_t(4 * S));
       }
       mma_commit<2>(done);
       mbar_wait(done, 0, nullptr, kMxWaitDone);
@@ -415,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
     const int row = 32 * q + lane;
     const uint32_t t_lane = tmem + (uint32_t(32 * q) << 16) + uint32_t(128 * half);
     const uint32_t out = base + uint32_t(Cfg::OFF_OUT + half * 128 * 128);
-    const uint32_t empty_bar = map_shared_rank(acc_empty, 0);
+    const uint32_t empty_bar = leader_bars + 8u * uint32_t(4 * S + 1);
     int n = 0;
     for (int t = pair; t < tiles; t += pairs, ++n) {
       if (!mbar_wait(acc_full, uint32_t(n) & 1u, abort_flag, kMxWaitAcc)) break;

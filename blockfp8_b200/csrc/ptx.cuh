@@ -488,12 +488,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 // 32 rows of 16 bytes from shared memory (512 contiguous bytes) into 4 TMEM
 // columns, the same 32 lanes repeated in each warp's quarter: the scale
-// factors of a 128-row x 128-column tile.  Ordered before MMAs that the same
-// thread issues after it.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-}
-// The same from each CTA of a pair into its own TMEM.
+// factors of a 128-row x 128-column tile, from each CTA of a pair into its own
+// TMEM.  Ordered before MMAs that the same thread issues after it.
 __device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t desc) {
   asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
 }
@@ -503,6 +499,17 @@ __device__ __forceinline__ void tmem_cp_scales_pair(uint32_t taddr, uint64_t des
 __device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
   return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(128 >> 4) << 32) | (uint64_t(1) << 46);
 }
+
+// 16 consecutive columns of this warp's 32 TMEM lanes from registers.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // D[tmem] (+)= (A * scale_A) (B * scale_B)^T over K = 64 e2m1 values, one
 // E8M0 scale per 32 (scale_vec::2X) from TMEM.
