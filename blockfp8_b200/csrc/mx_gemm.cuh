@@ -316,7 +316,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
   auto empty = [&](int s) { return bars + 8u * uint32_t(S + s); };
   auto sfull = [&](int s) { return bars + 8u * uint32_t(2 * S + s); };   // the leader's: both CTAs' scales
   auto scaled = [&](int s) { return bars + 8u * uint32_t(3 * S + s); };  // the leader's: they are in TMEM
-  const uint32_t leader_bars = map_shared_rank(bars, 0), peer_bars = map_shared_rank(bars, 1);
+  const uint32_t leader_bars = map_shared_rank(bars, 0);
   const uint32_t acc_full = bars + 8u * uint32_t(4 * S), acc_empty = acc_full + 8u, done = acc_full + 16u;
   const uint32_t copied = acc_full + 24u;
   uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BARS + 8 * (4 * S + 4));
@@ -433,6 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
         for (int k = 0; k < p.k_stages; ++k, ++i) {
           const int s = i % S;
           if (!(ok = mbar_wait(sfull(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull))) break;
+          if (!(ok = mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull))) break;  // for the MMAs
           tc_fence_after();
           const uint32_t sf = tmem + 256u + uint32_t(Cfg::SCALE_COLS * s);  // [kt][4 token, 8 weight columns]
           const uint64_t desc = smem_desc_scales(sx_tile(s));
@@ -451,29 +452,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
   } else if (warp == 1) {
     if (leader && lane == 0) {
       constexpr uint32_t idesc = idesc_mxf4(256, 256);
-      int i = 0, n = 0;
+      const uint64_t desc_a = smem_desc_k128_sw128(x_tile(0)), desc_b = smem_desc_k128_sw128(w_tile(0));
+      int n = 0, s = 0;
+      uint32_t phase = 0;
       bool ok = true;
       for (int t = pair; t < tiles && ok; t += pairs, ++n) {
         if (n > 0 && !mbar_wait(acc_empty, uint32_t(n - 1) & 1u, abort_flag, kMxWaitAcc)) break;
-        for (int k = 0; k < p.k_stages; ++k, ++i) {
-          const int s = i % S;
-          if (!(ok = mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull))) break;
-          if (!(ok = mbar_wait(scaled(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitScales))) break;
+        for (int left = p.K, first = 1; left > 0; left -= 256, first = 0) {
+          // (scaled: the codes have landed, too)
+          if (!(ok = mbar_wait(scaled(s), phase, abort_flag, kMxWaitScales))) break;
           tc_fence_after();
-          const int left = p.K - k * 256;
-          const int steps = left >= 256 ? 4 : (left + 63) / 64;
           const uint32_t sf = tmem + 256u + uint32_t(Cfg::SCALE_COLS * s);
-          const uint64_t a = smem_desc_k128_sw128(x_tile(s)), b = smem_desc_k128_sw128(w_tile(s));
+          const uint64_t a = desc_a + uint64_t(s * (2 * Cfg::TILE_BYTES >> 4)), b = desc_b + uint64_t(s * (2 * Cfg::TILE_BYTES >> 4));
+          auto mma = [&](int j) {  // K = 64 codes
+            mma_mxf4<2>(tmem, a + 2 * j, b + 2 * j, idesc | idesc_scale_half(j & 1), sf + uint32_t(12 * (j >> 1)),
+                        sf + uint32_t(12 * (j >> 1) + 4), j > 0 || !first);
+          };
+          if (left >= 256) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (j < steps)
-              mma_mxf4<2>(tmem, a + 2 * j, b + 2 * j, idesc | idesc_scale_half(j & 1), sf + uint32_t(12 * (j >> 1)),
-                          sf + uint32_t(12 * (j >> 1) + 4), (k > 0 || j > 0) ? 1u : 0u);
-          mma_commit<2>(empty(s));
-          mma_commit<2>(peer_bars + 8u * uint32_t(S + s));
+            for (int j = 0; j < 4; ++j) mma(j);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              if (64 * j < left) mma(j);
+          }
+          mma_commit_pair(empty(s));
+          if (++s == S) s = 0, phase ^= 1u;
         }
-        mma_commit<2>(acc_full);
-        mma_commit<2>(peer_bars + 8u * uint32_t(4 * S));
+        mma_commit_pair(acc_full);
       }
       mma_commit<2>(done);
       mbar_wait(done, 0, nullptr, kMxWaitDone);

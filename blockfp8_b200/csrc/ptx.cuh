@@ -381,6 +381,14 @@ __device__ __forceinline__ void mma_commit(uint32_t bar) {
                  : "memory");
 }
 
+// The same arrival on the barriers at one offset of both CTAs of a pair.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(static_cast<unsigned short>(3))
+      : "memory");
+}
+
 // 32 lanes x 32 consecutive 32-bit columns: thread i of the warp gets lane
 // (32 * (warp % 4) + i), columns [col, col + 32) of taddr.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
