@@ -96,7 +96,7 @@ int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaS
   if (!r) r = make_map(&gp.map_w, u8, p.b, uint64_t(p.K / 2), uint64_t(p.N), uint64_t(p.ldb), 128, 128, sw128);
   if (!r) r = make_map(&gp.map_sx, i32, p.sa, scale_row / 4, uint64_t(cdiv(p.M, 128)), scale_row, 256, 1, plain);
   if (!r) r = make_map(&gp.map_sw, i32, p.sb, scale_row / 4, uint64_t(cdiv(p.N, 128)), scale_row, 256, 2, plain);
-  if (!r) r = make_map(&gp.map_c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.c, uint64_t(p.N), uint64_t(p.M), uint64_t(p.ldc) * 2, 64, 128, sw128);
+  if (!r) r = make_map(&gp.map_c, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.c, uint64_t(p.N), uint64_t(p.M), uint64_t(p.ldc) * 2, 32, 128, CU_TENSOR_MAP_SWIZZLE_64B);
   if (r) return r;
   gp.K = p.K;
   gp.k_stages = cdiv(p.K, 256);

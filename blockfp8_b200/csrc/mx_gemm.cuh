@@ -58,6 +58,7 @@ enum MxWaitSite : uint32_t {
   kMxWaitDrain = 36,
   kMxWaitAcc = 37,
   kMxWaitScales = 38,
+  kMxLayout = 39,
 };
 
 template <int BN_, int STAGES_>
@@ -269,34 +270,36 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
 // There is no room for a second accumulator, so the epilogue first empties it
 // into registers as bf16 (eight warps, about 500 clocks of a tile's 8,192 at
 // K = 4096), frees it, and stores while the next tile runs: through shared
-// memory and TMA, 64 columns at a time.  Persistent, one pair on two SMs;
+// memory and TMA, 32 columns at a time.  Persistent, one pair on two SMs;
 // tiles go to the pairs in groups of eight token tiles, so that concurrent
 // tiles share operands in L2.
 //
-// Warps: 0 TMA producer of codes, 2 of scales, 1 MMA issuer and TMEM owner, 3
-// issuer of the scales' copies into TMEM (1 and 3 the leader's), 4-11 epilogue.
+// Warps: TMA producers 0 (weights), 12 (tokens) and 2 (scales), 1 MMA issuer and
+// TMEM owner, 3 issuer of the scales' copies into TMEM (1 and 3 the leader's),
+// 4-11 epilogue.
 struct MxPairParams {
   CUtensorMap map_x, map_w;    // codes [rows, K / 2] bytes: [128 x 128] boxes, 128-byte swizzle
   CUtensorMap map_sx, map_sw;  // scale tiles [row tiles, k_tiles * 512 bytes]: 1 and 2 x 1024 bytes
-  CUtensorMap map_c;           // C [M, N]: [128 x 64] boxes, 128-byte swizzle
+  CUtensorMap map_c;           // C [M, N]: [128 x 32] boxes, 64-byte swizzle
   int K, k_stages, m_tiles, n_tiles;  // tiles of 256
   int early;
 };
 
 struct MxPairCfg {
-  static constexpr int STAGES = 5;
-  static constexpr int THREADS = 384;
+  static constexpr int STAGES = 6;
+  static constexpr int THREADS = 416;
   static constexpr int TILE_BYTES = 128 * 128, S_BYTES = 1024;
   static constexpr int SCALE_COLS = 24;  // of a stage: [K tile][4 token, 8 weight columns]
-  static constexpr int OUT_BYTES = 2 * 128 * 128;                   // [column half][128 rows][64 bf16]
+  static constexpr int OUT_BYTES = 2 * 128 * 64;  // [column half][128 rows][32 bf16]
   static constexpr int TMEM_COLS = 512;
   // tiles stay 1024-byte aligned, scales behind all of them
   static constexpr int OFF_SCALES = STAGES * 2 * TILE_BYTES;
   static constexpr int OFF_OUT = OFF_SCALES + STAGES * 3 * S_BYTES;
-  static constexpr int OFF_BARS = OFF_OUT + OUT_BYTES;
   static_assert(OFF_OUT % 1024 == 0, "alignment");
-  static constexpr int SMEM_BYTES = 1024 + OFF_BARS + (4 * STAGES + 4) * 8 + 16;
   static_assert(256 + STAGES * SCALE_COLS <= TMEM_COLS, "TMEM");
+  // barriers in front, in what aligning the tiles to 1024 bytes leaves
+  static constexpr int BAR_BYTES = (4 * STAGES + 4) * 8 + 16;
+  static constexpr int SMEM_BYTES = 1024 + OFF_OUT + OUT_BYTES;
 };
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 1)
@@ -306,12 +309,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
   griddep_launch_dependents();
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
-  const uint32_t base = (raw + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (base - raw);
+  const uint32_t base = (raw + uint32_t(Cfg::BAR_BYTES) + 1023u) & ~1023u;
   auto x_tile = [&](int s) { return base + uint32_t(s * 2 * Cfg::TILE_BYTES); };
   auto w_tile = [&](int s) { return x_tile(s) + Cfg::TILE_BYTES; };
   auto sx_tile = [&](int s) { return base + uint32_t(Cfg::OFF_SCALES + s * 3 * Cfg::S_BYTES); };
-  const uint32_t bars = base + Cfg::OFF_BARS;
+  const uint32_t bars = raw;
   auto full = [&](int s) { return bars + 8u * uint32_t(s); };  // the leader's: both CTAs' copies
   auto empty = [&](int s) { return bars + 8u * uint32_t(S + s); };
   auto sfull = [&](int s) { return bars + 8u * uint32_t(2 * S + s); };   // the leader's: both CTAs' scales
@@ -319,9 +321,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
   const uint32_t leader_bars = map_shared_rank(bars, 0);
   const uint32_t acc_full = bars + 8u * uint32_t(4 * S), acc_empty = acc_full + 8u, done = acc_full + 16u;
   const uint32_t copied = acc_full + 24u;
-  uint32_t* misc = reinterpret_cast<uint32_t*>(smem + Cfg::OFF_BARS + 8 * (4 * S + 4));
+  uint32_t* misc = reinterpret_cast<uint32_t*>(smem_raw + 8 * (4 * S + 4));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(misc + 1);
 
+  if (base - raw > 1024u) {  // dynamic shared memory starts 1024-byte aligned: no static arrays here
+    record_status((0x5Bull << 56) | (uint64_t(kMxLayout) << 32));
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
   const bool leader = rank == 0;
@@ -362,21 +368,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
   tc_fence_after();
   const uint32_t tmem = misc[0];
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 12) {
+    // Weights (warp 0) and tokens (warp 12): a copy and the wait before it cost
+    // a thread about 250 clocks.
     if (lane == 0) {
+      const bool weights = warp == 0;
       const uint64_t pol = policy_evict_normal();
-      auto load_w = [&](int s, int k, int nt) {
-        if (leader) mbar_arrive_expect_tx(full(s), 4u * Cfg::TILE_BYTES);
-        tma_load_2d_pair(w_tile(s), &p.map_w, k * 128, nt * 256 + int(rank) * 128, leader_bars + 8u * uint32_t(s), pol);
-      };
-      auto load_x = [&](int s, int k, int mt) {
-        tma_load_2d_pair(x_tile(s), &p.map_x, k * 128, mt * 256 + int(rank) * 128, leader_bars + 8u * uint32_t(s), pol);
+      auto load = [&](int s, int k, int mt, int nt) {
+        const uint32_t bar = leader_bars + 8u * uint32_t(s);
+        if (weights) {
+          if (leader) mbar_arrive_expect_tx(full(s), 4u * Cfg::TILE_BYTES);
+          tma_load_2d_pair(w_tile(s), &p.map_w, k * 128, nt * 256 + int(rank) * 128, bar, pol);
+        } else {
+          tma_load_2d_pair(x_tile(s), &p.map_x, k * 128, mt * 256 + int(rank) * 128, bar, pol);
+        }
       };
       int pre = 0;
-      if (p.early && pair < tiles) {
+      if (weights && p.early && pair < tiles) {
         int mt, nt;
         place(pair, mt, nt);
-        for (; pre < S && pre < p.k_stages; ++pre) load_w(pre, pre, nt);
+        for (; pre < S && pre < p.k_stages; ++pre) load(pre, pre, mt, nt);
       }
       griddep_wait();
       int i = 0;
@@ -387,8 +398,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
         for (int k = 0; k < p.k_stages; ++k, ++i) {
           const int s = i % S;
           if (i >= S && !(ok = mbar_wait(empty(s), uint32_t(i / S - 1) & 1u, abort_flag, kMxWaitEmpty))) break;
-          if (i >= pre) load_w(s, k, nt);
-          load_x(s, k, mt);
+          if (i >= pre) load(s, k, mt, nt);
         }
       }
       // The leader's MMAs read what was loaded last; every copy has landed once
@@ -485,12 +495,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
       mbar_wait(done, 0, nullptr, kMxWaitDone);
     }
     __syncwarp();
-  } else if (warp >= 4) {
+  } else {
     griddep_wait();  // C
     const int q = warp & 3, half = (warp - 4) >> 2;  // lanes 32 q .., columns 128 half ..
     const int row = 32 * q + lane;
     const uint32_t t_lane = tmem + (uint32_t(32 * q) << 16) + uint32_t(128 * half);
-    const uint32_t out = base + uint32_t(Cfg::OFF_OUT + half * 128 * 128);
+    const uint32_t out = base + uint32_t(Cfg::OFF_OUT + half * 128 * 64);
     const uint32_t empty_bar = leader_bars + 8u * uint32_t(4 * S + 1);
     int n = 0;
     for (int t = pair; t < tiles; t += pairs, ++n) {
@@ -513,17 +523,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
       int mt, nt;
       place(t, mt, nt);
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {  // 64 columns: 128 bytes a row
+      for (int c = 0; c < 4; ++c) {  // 32 columns: 64 bytes a row, in the 64-byte swizzle
         // the store that read this buffer last is done
         if ((warp & 3) == 0 && lane == 0) bulk_wait_read0();
         named_bar_sync(1 + half, 128);
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          st_shared_v4(out + uint32_t(row * 128 + ((j ^ (row & 7)) << 4)), packed[c * 32 + 4 * j], packed[c * 32 + 4 * j + 1],
-                       packed[c * 32 + 4 * j + 2], packed[c * 32 + 4 * j + 3]);
+        for (int j = 0; j < 4; ++j)
+          st_shared_v4(out + uint32_t(row * 64 + ((j ^ ((row >> 1) & 3)) << 4)), packed[c * 16 + 4 * j],
+                       packed[c * 16 + 4 * j + 1], packed[c * 16 + 4 * j + 2], packed[c * 16 + 4 * j + 3]);
         fence_proxy_async_smem();
         named_bar_sync(1 + half, 128);
-        const int col = nt * 256 + half * 128 + c * 64;
+        const int col = nt * 256 + half * 128 + c * 32;
         if ((warp & 3) == 0 && lane == 0 && !*abort_flag) {
           tma_store_2d(&p.map_c, col, mt * 256 + int(rank) * 128, out);
           bulk_commit();
