@@ -83,7 +83,7 @@ class Mxfp4QuantProblem(ctypes.Structure):
     _fields_ = [
         ("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("x_type", ctypes.c_int),
         ("q", ctypes.c_void_p), ("ldq", ctypes.c_int64), ("s", ctypes.c_void_p),
-        ("M", ctypes.c_int), ("K", ctypes.c_int),
+        ("M", ctypes.c_int), ("K", ctypes.c_int), ("trigger", ctypes.c_int),
     ]
 
 
@@ -103,6 +103,7 @@ class Mxfp4GemmProblem(ctypes.Structure):
         ("b", ctypes.c_void_p), ("ldb", ctypes.c_int64), ("sb", ctypes.c_void_p),
         ("c", ctypes.c_void_p), ("ldc", ctypes.c_int64),
         ("M", ctypes.c_int), ("N", ctypes.c_int), ("K", ctypes.c_int), ("weights_ready", ctypes.c_int),
+        ("a_type", ctypes.c_int),
     ]
 
 

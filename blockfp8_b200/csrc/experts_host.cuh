@@ -18,6 +18,8 @@ int allow_smem(const void* kernel, int bytes, int dev, std::atomic<uint64_t>& do
 
 int element_size(int type) { return type == 0 ? 4 : 2; }
 
+int round_up(int x, int m) { return cdiv(x, m) * m; }
+
 // ---- MXFP4 quantization -----------------------------------------------------------
 
 int check_codes(const void* q, int64_t ldq, const void* s, int M, int K) {
@@ -46,34 +48,65 @@ int launch_mx(const void* kernel, int m_tiles, int k_tiles, void** args, int num
 
 // ---- MXFP4 GEMM -------------------------------------------------------------------
 
+constexpr int kMxPairSmem = 112 * 1024;  // two CTAs on an SM
+
+// K parts of a tile: more while the CTAs still fit two to an SM and each has
+// two stages.
+int mx_splits(int64_t tiles, int k_stages, int num_sms) {
+  int splits = 1;
+  while (splits < 8 && tiles * splits <= num_sms && k_stages >= splits * 4) splits *= 2;
+  return splits;
+}
+
 template <class Cfg>
-int launch_mx_gemm(MxGemmParams& gp, const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaStream_t stream) {
+int launch_mx_gemm(const bfp8_mxfp4_gemm_problem& p, int x_type, int dev, int num_sms, cudaStream_t stream) {
   static std::atomic<uint64_t> done{0};
   const void* kernel = reinterpret_cast<const void*>(&mx_gemm_kernel<Cfg>);
-  if (int r = allow_smem(kernel, Cfg::SMEM_BYTES, dev, done)) return r;
+  if (int r = allow_smem(kernel, kMxPairSmem, dev, done)) return r;
+  MxGemmParams gp;
+  std::memset(&gp, 0, sizeof(gp));
   if (int r = make_map(&gp.map_w, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.b, uint64_t(p.K / 2), uint64_t(p.N), uint64_t(p.ldb),
                        128, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return r;
-  if (int r = make_map(&gp.map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, uint64_t(p.K / 2), uint64_t(p.M), uint64_t(p.lda),
-                       128, Cfg::BN, CU_TENSOR_MAP_SWIZZLE_128B))
-    return r;
+  if (Cfg::QUANT) {
+    if (int r = make_map(&gp.map_x, CU_TENSOR_MAP_DATA_TYPE_UINT16, p.a, uint64_t(p.K), uint64_t(p.M),
+                         uint64_t(p.lda) * 2, 256, uint32_t(p.M), CU_TENSOR_MAP_SWIZZLE_NONE))
+      return r;
+  } else {
+    if (int r = make_map(&gp.map_x, CU_TENSOR_MAP_DATA_TYPE_UINT8, p.a, uint64_t(p.K / 2), uint64_t(p.M),
+                         uint64_t(p.lda), 128, Cfg::BN, CU_TENSOR_MAP_SWIZZLE_128B))
+      return r;
+  }
+  gp.sw = static_cast<const uint8_t*>(p.sb);
+  gp.sx = static_cast<const uint8_t*>(p.sa);
+  gp.c = static_cast<__nv_bfloat16*>(p.c);
+  gp.ldc = p.ldc;
+  gp.M = p.M;
+  gp.N = p.N;
+  gp.K = p.K;
+  gp.n_tiles = cdiv(p.N, 128);
   gp.m_tiles = cdiv(p.M, Cfg::BN);
+  gp.k_tiles = cdiv(p.K, 128);
+  gp.k_stages = cdiv(p.K, 256);
+  gp.early = p.weights_ready && g_weight_prefetch.load(std::memory_order_relaxed);
+  gp.half = x_type == 2;
+  gp.raw_bytes = Cfg::QUANT ? p.M * 512 : 0;
+  gp.stage_bytes = round_up(Cfg::TILE_BYTES + gp.raw_bytes, 1024);
+  gp.stages = std::min(Cfg::MAX_STAGES, (kMxPairSmem - 1024 - Cfg::BAR_BYTES) / gp.stage_bytes);
+  const int smem = 1024 + std::max(gp.stages * gp.stage_bytes, Cfg::SUM_BYTES) + Cfg::BAR_BYTES;
   const int64_t tiles = int64_t(gp.n_tiles) * gp.m_tiles;
-  // K parts while the CTAs still fit two to an SM and each has two stages.
-  int splits = 1;
-  while (splits < 8 && tiles * splits * 2 <= 2 * int64_t(num_sms) && gp.k_stages >= splits * 4) splits *= 2;
-  gp.splits = splits;
-  if (tiles * splits > INT32_MAX) return fail(BFP8_EINVAL, "too many tiles for one launch");
+  gp.splits = mx_splits(tiles, gp.k_stages, num_sms);
+  if (tiles * gp.splits > INT32_MAX) return fail(BFP8_EINVAL, "too many tiles for one launch");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(tiles * splits));
+  cfg.gridDim = dim3(unsigned(tiles * gp.splits));
   cfg.blockDim = dim3(Cfg::THREADS);
-  cfg.dynamicSmemBytes = Cfg::SMEM_BYTES;
+  cfg.dynamicSmemBytes = size_t(smem);
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
   set_pdl(cfg, attr);
-  if (splits > 1) {
+  if (gp.splits > 1) {
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = unsigned(splits);
+    attr[1].val.clusterDim.x = unsigned(gp.splits);
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
   }
@@ -102,7 +135,7 @@ int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaS
   gp.k_stages = cdiv(p.K, 256);
   gp.m_tiles = cdiv(p.M, 256);
   gp.n_tiles = cdiv(p.N, 256);
-  gp.early = p.weights_ready ? 1 : 0;
+  gp.early = p.weights_ready && g_weight_prefetch.load(std::memory_order_relaxed);
   const int64_t tiles = int64_t(gp.m_tiles) * gp.n_tiles;
   if (tiles > INT32_MAX / 8) return fail(BFP8_EINVAL, "too many tiles for one launch");
   cudaLaunchConfig_t cfg{};
@@ -123,8 +156,6 @@ int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaS
 constexpr int kMoeMaxHidden = 8192;
 constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
 constexpr int kMoeHalfSmem = 113 * 1024;
-
-int round_up(int x, int m) { return cdiv(x, m) * m; }
 
 // How one kernel's units (segments of seg_len values of K) and shared memory
 // are laid out.
@@ -334,9 +365,9 @@ int bfp8_launch_mxfp4_quantize(const bfp8_mxfp4_quant_problem* pp, void* stream)
     return fail(BFP8_EINVAL, "x must be row-major with 16-byte aligned rows");
   int dev = 0;
   const int num_sms = current_device_sms(&dev);
-  if (num_sms < 0) return num_sms;
+  if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");
   Mxfp4QuantParams k{p.x, p.ldx, static_cast<uint8_t*>(p.q), p.ldq, static_cast<uint8_t*>(p.s), p.M, p.K,
-                     cdiv(p.M, 128), cdiv(p.K, 128)};
+                     cdiv(p.M, 128), cdiv(p.K, 128), p.trigger ? 1 : 0};
   void* args[] = {&k};
   const void* kernel = p.x_type == 0   ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<float>)
                        : p.x_type == 1 ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<__nv_bfloat16>)
@@ -355,7 +386,7 @@ int bfp8_launch_mxfp4_dequantize(const bfp8_mxfp4_dequant_problem* pp, void* str
     return fail(BFP8_EINVAL, "y must be row-major with 16-byte aligned rows");
   int dev = 0;
   const int num_sms = current_device_sms(&dev);
-  if (num_sms < 0) return num_sms;
+  if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");
   Mxfp4DequantParams k{static_cast<const uint8_t*>(p.q), p.ldq, static_cast<const uint8_t*>(p.s), p.y, p.ldy, p.M, p.K,
                        cdiv(p.M, 128), cdiv(p.K, 128)};
   void* args[] = {&k};
@@ -368,35 +399,40 @@ int bfp8_launch_mxfp4_dequantize(const bfp8_mxfp4_dequant_problem* pp, void* str
 int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* pp, void* stream) {
   if (!pp) return fail(BFP8_EINVAL, "null problem");
   const bfp8_mxfp4_gemm_problem& p = *pp;
+  const bool quant = p.a_type != 0;  // 16-bit activations
   if (p.N <= 0 || p.N % 8) return fail(BFP8_EINVAL, "N must be a positive multiple of 8");
-  if (int r = check_codes(p.a, p.lda, p.sa, p.M, p.K)) return r;
+  if (p.a_type < 0 || p.a_type > 2) return fail(BFP8_EINVAL, "a must be MXFP4 codes, bf16 or fp16");
+  if (quant) {
+    if (p.M < 0 || p.M > BFP8_MXFP4_QUANT_MAX_M || p.K <= 0 || p.K % 32)
+      return fail(BFP8_EINVAL, "16-bit activations: at most 16 rows, K a positive multiple of 32");
+    if (p.M && (!p.a || !aligned16(p.a) || p.lda < p.K || p.lda % 8))
+      return fail(BFP8_EINVAL, "a must be row-major with 16-byte aligned rows");
+  } else if (int r = check_codes(p.a, p.lda, p.sa, p.M, p.K)) {
+    return r;
+  }
   if (p.M == 0) return BFP8_OK;
   if (int r = check_codes(p.b, p.ldb, p.sb, p.N, p.K)) return r;
   if (!p.c || !aligned16(p.c) || p.ldc < p.N || p.ldc % 8)
     return fail(BFP8_EINVAL, "c must be row-major with 8-element aligned rows");
   int dev = 0;
   const int num_sms = current_device_sms(&dev);
-  if (num_sms < 0) return num_sms;
-  MxGemmParams gp;
-  std::memset(&gp, 0, sizeof(gp));
-  gp.sw = static_cast<const uint8_t*>(p.sb);
-  gp.sx = static_cast<const uint8_t*>(p.sa);
-  gp.c = static_cast<__nv_bfloat16*>(p.c);
-  gp.ldc = p.ldc;
-  gp.M = p.M;
-  gp.N = p.N;
-  gp.K = p.K;
-  gp.n_tiles = cdiv(p.N, 128);
-  gp.k_tiles = cdiv(p.K, 128);
-  gp.k_stages = cdiv(p.K, 256);
-  gp.early = p.weights_ready ? 1 : 0;
+  if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (p.M <= 16) return launch_mx_gemm<MxCfg<16, 5>>(gp, p, dev, num_sms, s);
-  if (p.M <= 32) return launch_mx_gemm<MxCfg<32, 5>>(gp, p, dev, num_sms, s);
-  if (p.M <= 64) return launch_mx_gemm<MxCfg<64, 4>>(gp, p, dev, num_sms, s);
-  // Pairs once their tiles fill the GPU.
-  if (int64_t(cdiv(p.M, 256)) * cdiv(p.N, 256) >= num_sms / 2) return launch_mx_pair(p, dev, num_sms, s);
-  return launch_mx_gemm<MxCfg<128, 3>>(gp, p, dev, num_sms, s);
+  if (quant) return launch_mx_gemm<MxCfg<16, true>>(p, p.a_type, dev, num_sms, s);
+  if (p.M <= 16) return launch_mx_gemm<MxCfg<16, false>>(p, 0, dev, num_sms, s);
+  if (p.M <= 32) return launch_mx_gemm<MxCfg<32, false>>(p, 0, dev, num_sms, s);
+  if (p.M <= 64) return launch_mx_gemm<MxCfg<64, false>>(p, 0, dev, num_sms, s);
+  // Beyond a token tile: pairs, or single CTAs with K split, whichever this
+  // fit to measured times (us) puts ahead.  Measured, single and pairs: 256 x
+  // 6144 x 4096 14.3 and 11.9, 256 x 24576 x 4096 31.9 and 20.6, 256 x 4096 x
+  // 12288 14.9 and 25.0, 512 x 6144 x 4096 15.6 and 12.9.
+  const int k_stages = cdiv(p.K, 256);
+  const int64_t tiles = int64_t(cdiv(p.N, 128)) * cdiv(p.M, 128), splits = mx_splits(tiles, k_stages, num_sms);
+  const int64_t rounds = (int64_t(cdiv(p.N, 256)) * cdiv(p.M, 256) + num_sms / 2 - 1) / (num_sms / 2);
+  const double single = 4 + 1.35 * double(cdiv(k_stages, int(splits))) * std::max(0.65, double(tiles * splits) / (2 * num_sms));
+  const double paired = 2.4 + double(rounds) * (0.55 * k_stages + 0.7);
+  if (p.M > 128 && paired < single) return launch_mx_pair(p, dev, num_sms, s);
+  return launch_mx_gemm<MxCfg<128, false>>(p, 0, dev, num_sms, s);
 }
 
 int64_t bfp8_moe_workspace_bytes(const bfp8_moe_problem* pp) {
@@ -418,7 +454,7 @@ int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
   if (!moe_shape(p, &s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
   int dev = 0;
   const int num_sms = current_device_sms(&dev);
-  if (num_sms < 0) return num_sms;
+  if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");
   const int64_t pairs = int64_t(p.T) * p.top_k;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   MoeParams mp;

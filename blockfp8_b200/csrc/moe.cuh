@@ -165,7 +165,9 @@ __device__ __forceinline__ void moe_top_k(const MoeParams& p, const MoeRoute& r,
       if (key[i] >= best) best = key[i], at = uint32_t(i * 32 + lane);
     const uint32_t most = __reduce_max_sync(~0u, best);
     if (most == 0u) break;  // nothing left to choose
-    id = int(__reduce_min_sync(~0u, best == most ? at : ~0u));
+    const uint32_t who = __ballot_sync(~0u, best == most);
+    id = who & (who - 1u) ? int(__reduce_min_sync(~0u, best == most ? at : ~0u))  // equals: the lowest index
+                          : int(__shfl_sync(~0u, at, __ffs(who) - 1));
     const float v = moe_key_value(most);
     if (j == 0) {
       top = v;
@@ -527,36 +529,44 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   auto fragments = [&](int columns, int k_len, auto row_of) {  // by the consumer warps
     const int blocks = (k_len + 127) / 128, tasks = columns * blocks;
     const int half = tid >> 4, l16 = tid & 15;  // a half-warp's task is one column's block
-    for (int task0 = 0; task0 < tasks; task0 += 2 * W) {
-      const int task = task0 + half;
-      const int col = task / blocks, b = task - col * blocks;
-      const int k = b * 128 + l16 * 8;
-      float v[8];
+    constexpr int U = 2;  // tasks whose loads are in flight together
+    for (int task0 = 0; task0 < tasks; task0 += 2 * W * U) {
+      float v[U][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      if (task < tasks && k < k_len) load8(row_of(col) + k, v);
-      uint32_t m = 0u;
+      for (int u = 0; u < U; ++u) {
+        const int task = task0 + u * 2 * W + half;
+        const int col = task / blocks, k = (task - col * blocks) * 128 + l16 * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+        for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+        if (task < tasks && k < k_len) load8(row_of(col) + k, v[u]);
+      }
 #pragma unroll
-      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
-      float to, back;
-      moe_act_scale(m, to, back);
-      if (task < tasks) {
-        uint32_t w[4];
+      for (int u = 0; u < U; ++u) {
+        const int task = task0 + u * 2 * W + half;
+        const int col = task / blocks, b = task - col * blocks;
+        uint32_t m = 0u;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v[2 * i] * to, v[2 * i + 1] * to);
-        uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + col * 64;
-        if constexpr (MX) {
-          // a lane's codes are 8 consecutive values
-          *reinterpret_cast<uint4*>(to16 + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-        } else {
-          // a lane's codes are 4 consecutive values of each 16
-          uint8_t* at = to16 + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
-          *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-          *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[u][i]) & 0x7FFFFFFFu);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(~0u, m, o));
+        float to, back;
+        moe_act_scale(m, to, back);
+        if (task < tasks) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v[u][2 * i] * to, v[u][2 * i + 1] * to);
+          uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + col * 64;
+          if constexpr (MX) {
+            // a lane's codes are 8 consecutive values
+            *reinterpret_cast<uint4*>(to16 + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+          } else {
+            // a lane's codes are 4 consecutive values of each 16
+            uint8_t* at = to16 + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
+            *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+            *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
+          }
+          if (l16 == 0) ts[b * 8 * NT + col] = back;
         }
-        if (l16 == 0) ts[b * 8 * NT + col] = back;
       }
     }
   };
@@ -671,7 +681,6 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
     uint32_t b_lane[NT];
 #pragma unroll
     for (int c = 0; c < NT; ++c) b_lane[c] = base + p.off_b + uint32_t(min(c * 8 + g, p.cols - 1) * 64 + t4 * 16);
-    if constexpr (!GATE) griddep_wait();  // h
     constexpr int kStep = Cfg::GROUP_WARPS;
     const int group = warp / kStep, warp_in_group = warp % kStep;
     const uint32_t a_lane = ((lane >> 3) & 1) * half_bytes + (lane & 7) * 128u;
@@ -696,6 +705,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
     };
     Walk w = begin();
     if (!MX && w.u < u1 && group < w.count) load_scales(w.chunk, w.seg, w.tile + group);
+    if constexpr (!GATE) griddep_wait();  // h
     for (; w.u < u1; next(w)) {
       const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
       const int k_len = min(p.seg_len, K - seg * p.seg_len);

@@ -37,6 +37,7 @@ struct Mxfp4QuantParams {
   uint8_t* s;  // [m_tiles, k_tiles, 32, 16]
   int M, K;
   int m_tiles, k_tiles;
+  int trigger;  // let the dependent kernel start early (it waits before it reads q and s)
 };
 
 struct Mxfp4DequantParams {
@@ -103,6 +104,12 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   }
 }
 
+// The scale byte of a block from the bits of its largest magnitude.
+__device__ __forceinline__ uint32_t mxfp4_scale_byte(uint32_t amax_bits) {
+  const uint32_t ef = amax_bits >> 23;  // floor(log2) + 127; 0 for subnormals
+  return ef == 255u ? 255u : (ef > 2u ? ef - 2u : 0u);
+}
+
 constexpr int kMxThreads = 256;
 
 // A warp takes rows r, r + 32, r + 64, r + 96 of a 128-row tile over 256
@@ -112,9 +119,11 @@ constexpr int kMxThreads = 256;
 template <class T>
 __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4QuantParams p) {
   // The wait comes first: a dependent that has started may then read whatever
-  // earlier kernels wrote (the GEMM of linear_mxfp4 its weights) at once.
+  // earlier kernels wrote (the GEMM of linear_mxfp4 its weights) at once.  As
+  // this kernel may be the one that writes such weights, it triggers only
+  // inside linear_mxfp4.
   griddep_wait();
-  griddep_launch_dependents();
+  if (p.trigger) griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int chunks = (p.k_tiles + 1) / 2;
   const int64_t tasks = int64_t(p.m_tiles) * 32 * chunks;
@@ -126,7 +135,6 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4Q
     const int col = chunk * 256 + lane * 8;
     const bool col_ok = col < p.K;
     float v[4][8];
-    uint32_t amax[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = mt * 128 + r + 32 * j;
@@ -143,9 +151,7 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4Q
       for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[j][i]) & 0x7FFFFFFFu);
       m = max(m, __shfl_xor_sync(~0u, m, 1));
       m = max(m, __shfl_xor_sync(~0u, m, 2));
-      amax[j] = m;
-      const uint32_t ef = m >> 23;  // floor(log2) + 127; 0 for subnormals
-      bytes[j] = ef == 255u ? 255u : (ef > 2u ? ef - 2u : 0u);
+      bytes[j] = mxfp4_scale_byte(m);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {

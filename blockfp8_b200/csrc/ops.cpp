@@ -398,9 +398,9 @@ void check_mxfp4_input(const at::Tensor& x, const char* op) {
   CHECK_VALUE(aligned_rows(x), op, ": x must be row-major with 16-byte aligned rows, got strides ", x.strides());
 }
 
-void launch_mxfp4_quantize(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s) {
-  const bfp8_mxfp4_quant_problem p{x.data_ptr(), row_stride(x),  float_type(x),     q.data_ptr(),
-                                   row_stride(q), s.data_ptr(), int(x.size(0)), int(x.size(1))};
+void launch_mxfp4_quantize(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s, bool trigger) {
+  const bfp8_mxfp4_quant_problem p{x.data_ptr(),  row_stride(x), float_type(x),  q.data_ptr(),
+                                   row_stride(q), s.data_ptr(),  int(x.size(0)), int(x.size(1)), trigger ? 1 : 0};
   require_abi(bfp8_launch_mxfp4_quantize(&p, at::cuda::getCurrentCUDAStream().stream()));
 }
 
@@ -412,7 +412,7 @@ std::tuple<at::Tensor, at::Tensor> quantize_mxfp4(const at::Tensor& x) {
   check_cuda({&x}, op);
   const at::cuda::CUDAGuard guard(x.device());
   auto out = empty_mxfp4(x, x.size(0), x.size(1));
-  if (x.size(0) > 0) launch_mxfp4_quantize(x, std::get<0>(out), std::get<1>(out));
+  if (x.size(0) > 0) launch_mxfp4_quantize(x, std::get<0>(out), std::get<1>(out), false);
   return out;
 }
 
@@ -430,12 +430,15 @@ at::Tensor dequantize_mxfp4(const at::Tensor& q, const at::Tensor& s, at::Scalar
   return y;
 }
 
-at::Tensor launch_mxfp4_gemm(const at::Tensor& a, const at::Tensor& sa, const at::Tensor& b, const at::Tensor& sb,
+// a: codes with their scales, or (sa null) 16-bit activations.
+at::Tensor launch_mxfp4_gemm(const at::Tensor& a, const at::Tensor* sa, const at::Tensor& b, const at::Tensor& sb,
                              bool weights_ready) {
   at::Tensor c = at::empty({a.size(0), b.size(0)}, a.options().dtype(at::kBFloat16));
-  const bfp8_mxfp4_gemm_problem p{a.data_ptr(),   row_stride(a),  sa.data_ptr(),   b.data_ptr(),
-                                  row_stride(b),  sb.data_ptr(),  c.data_ptr(),    c.stride(0),
-                                  int(a.size(0)), int(b.size(0)), int(2 * a.size(1)), weights_ready ? 1 : 0};
+  const bfp8_mxfp4_gemm_problem p{a.data_ptr(),   row_stride(a),
+                                  sa ? sa->data_ptr() : nullptr,
+                                  b.data_ptr(),   row_stride(b),  sb.data_ptr(),      c.data_ptr(),
+                                  c.stride(0),    int(a.size(0)), int(b.size(0)),     int(2 * b.size(1)),
+                                  weights_ready ? 1 : 0, sa ? 0 : float_type(a)};
   require_abi(bfp8_launch_mxfp4_gemm(&p, at::cuda::getCurrentCUDAStream().stream()));
   return c;
 }
@@ -454,12 +457,14 @@ at::Tensor gemm_mxfp4(const at::Tensor& a, const at::Tensor& a_scales, const at:
   const at::cuda::CUDAGuard guard(a.device());
   if (a.size(0) == 0) return at::empty({0, b.size(0)}, a.options().dtype(at::kBFloat16));
   // b may have been written by the kernel right before this one
-  return launch_mxfp4_gemm(a, a_scales, b, b_scales, false);
+  return launch_mxfp4_gemm(a, &a_scales, b, b_scales, false);
 }
 
-// quantize_mxfp4 then gemm_mxfp4.  The GEMM may request its weights while the
-// quantization kernel runs, which starts (and lets the GEMM start) only after
-// every earlier kernel has finished.
+// quantize_mxfp4 then gemm_mxfp4; in one kernel for up to 16 tokens while the
+// weight tiles are no more than the SMs (each quantizes again).  The GEMM
+// may request its weights as soon as it starts: the quantization kernel lets it
+// start only after every earlier kernel has finished, and quantize_mxfp4 (which
+// may just have written them) not before its own end.
 at::Tensor linear_mxfp4(const at::Tensor& x, const at::Tensor& b, const at::Tensor& b_scales) {
   const char* op = "blockfp8_b200.linear_mxfp4";
   CHECK_VALUE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, op,
@@ -469,9 +474,11 @@ at::Tensor linear_mxfp4(const at::Tensor& x, const at::Tensor& b, const at::Tens
   check_cuda({&x, &b, &b_scales}, op);
   const at::cuda::CUDAGuard guard(x.device());
   if (x.size(0) == 0) return at::empty({0, b.size(0)}, x.options().dtype(at::kBFloat16));
+  if (x.size(0) <= BFP8_MXFP4_QUANT_MAX_M && cdiv(b.size(0), 128) <= sm_count())
+    return launch_mxfp4_gemm(x, nullptr, b, b_scales, true);
   const auto [q, s] = empty_mxfp4(x, x.size(0), x.size(1));
-  launch_mxfp4_quantize(x, q, s);
-  return launch_mxfp4_gemm(q, s, b, b_scales, true);
+  launch_mxfp4_quantize(x, q, s, true);
+  return launch_mxfp4_gemm(q, &s, b, b_scales, true);
 }
 
 // One of the layer's two weight stacks: [E, rows, K] in either format.

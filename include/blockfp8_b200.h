@@ -283,7 +283,9 @@ int bfp8_launch_silu_mul_quant(const bfp8_silu_mul_quant_problem* p, void* strea
  * bytes at 4 (r / 32); bytes past the matrix are zero.  K is a multiple of
  * 32; rows of codes are 16-byte aligned. */
 
-/* x [M, K] (x_type 0: fp32, 1: bf16, 2: fp16; rows 16-byte aligned) -> q, s. */
+/* x [M, K] (x_type 0: fp32, 1: bf16, 2: fp16; rows 16-byte aligned) -> q, s.
+ * trigger != 0: the next kernel of the stream may start while this one runs
+ * (one that waits before it reads q and s, as bfp8_launch_mxfp4_gemm does). */
 typedef struct bfp8_mxfp4_quant_problem {
   const void* x;
   int64_t ldx;
@@ -292,6 +294,7 @@ typedef struct bfp8_mxfp4_quant_problem {
   int64_t ldq; /* bytes */
   void* s;
   int M, K;
+  int trigger;
 } bfp8_mxfp4_quant_problem;
 int bfp8_launch_mxfp4_quantize(const bfp8_mxfp4_quant_problem* p, void* stream);
 
@@ -308,12 +311,15 @@ typedef struct bfp8_mxfp4_dequant_problem {
 int bfp8_launch_mxfp4_dequantize(const bfp8_mxfp4_dequant_problem* p, void* stream);
 
 /* C [M, N] bf16 = A [M, K] B [N, K]^T, both MXFP4, accumulated in fp32.  N a
- * multiple of 8.  weights_ready != 0: every kernel that wrote b or sb has
- * finished before the kernel ahead of this one in the stream started (then
- * they are requested while that kernel still runs). */
+ * multiple of 8.  a_type 0: a and sa are MXFP4; 1 or 2: a is bf16 or fp16 with
+ * at most BFP8_MXFP4_QUANT_MAX_M rows, lda counts elements, and the kernel
+ * quantizes it as bfp8_launch_mxfp4_quantize does (sa unused).  weights_ready
+ * != 0: no kernel that still runs when this one may start (see trigger) writes
+ * b or sb; they are then requested at once (bfp8_set_weight_prefetch). */
+#define BFP8_MXFP4_QUANT_MAX_M 16
 typedef struct bfp8_mxfp4_gemm_problem {
   const void* a;
-  int64_t lda; /* bytes */
+  int64_t lda; /* bytes; a_type != 0: elements */
   const void* sa;
   const void* b;
   int64_t ldb;
@@ -322,6 +328,7 @@ typedef struct bfp8_mxfp4_gemm_problem {
   int64_t ldc;
   int M, N, K;
   int weights_ready;
+  int a_type;
 } bfp8_mxfp4_gemm_problem;
 int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* p, void* stream);
 

@@ -107,7 +107,7 @@ def _integers(rows, k, seed):
 
 SHAPES = [
     (1, 8, 32), (1, 128, 64), (2, 136, 96), (5, 256, 128), (7, 1000, 160), (16, 6144, 4096), (17, 384, 288),
-    (24, 4096, 12288), (32, 520, 512), (33, 256, 2080), (64, 1024, 1024), (65, 512, 768), (128, 640, 544),
+    (8, 20000, 96), (24, 4096, 12288), (32, 520, 512), (33, 256, 2080), (64, 1024, 1024), (65, 512, 768), (128, 640, 544),
     (129, 264, 4128), (200, 2048, 352), (256, 256, 256), (257, 1032, 1312), (509, 6120, 4128), (1000, 776, 1056),
     (2048, 1536, 512), (2500, 2056, 800), (1030, 8200, 1440),
 ]
