@@ -34,6 +34,7 @@ int check_codes(const void* q, int64_t ldq, const void* s, int M, int K) {
 int launch_mx(const void* kernel, int m_tiles, int k_tiles, void** args, int num_sms, cudaStream_t stream,
               const char* what) {
   const int64_t tasks = int64_t(m_tiles) * 32 * cdiv(k_tiles, 2);
+  if (tasks > INT32_MAX) return fail(BFP8_EINVAL, "too many rows x columns for one launch");
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(std::min<int64_t>((tasks + kMxThreads / 32 - 1) / (kMxThreads / 32), int64_t(num_sms) * 16)));
   cfg.blockDim = dim3(kMxThreads);

@@ -126,12 +126,10 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4Q
   if (p.trigger) griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int chunks = (p.k_tiles + 1) / 2;
-  const int64_t tasks = int64_t(p.m_tiles) * 32 * chunks;
-  const int64_t warps = int64_t(gridDim.x) * (kMxThreads / 32);
-  for (int64_t task = int64_t(blockIdx.x) * (kMxThreads / 32) + (threadIdx.x >> 5); task < tasks; task += warps) {
-    const int chunk = int(task % chunks);
-    const int64_t rows = task / chunks;  // (row tile, r)
-    const int r = int(rows & 31), mt = int(rows >> 5);
+  const uint32_t tasks = uint32_t(p.m_tiles) * 32u * uint32_t(chunks), warps = gridDim.x * (kMxThreads / 32);
+  for (uint32_t task = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); task < tasks; task += warps) {
+    const int rows = int(task / uint32_t(chunks)), chunk = int(task) - rows * chunks;  // (row tile, r)
+    const int r = rows & 31, mt = rows >> 5;
     const int col = chunk * 256 + lane * 8;
     const bool col_ok = col < p.K;
     float v[4][8];
@@ -156,12 +154,12 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4Q
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int row = mt * 128 + r + 32 * j;
-      const float inv = bytes[j] == 255u ? 0.f : e8m0_inverse(bytes[j]);
+      const float inv = e8m0_inverse(min(bytes[j], 253u));
       float w[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = bytes[j] == 255u ? 0.f : v[j][i] * inv;
+      for (int i = 0; i < 8; ++i) w[i] = v[j][i] * inv;
       if (col_ok && row < p.M)
-        *reinterpret_cast<uint32_t*>(p.q + int64_t(row) * p.ldq + col / 2) = e2m1x8(w);
+        *reinterpret_cast<uint32_t*>(p.q + int64_t(row) * p.ldq + col / 2) = bytes[j] == 255u ? 0u : e2m1x8(w);
     }
     // 16 scale bytes of a K tile from its 16 lanes: lane 4 b holds block b.
     uint32_t word[4];
@@ -187,12 +185,10 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_dequantize_kernel(const Mxfp
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int chunks = (p.k_tiles + 1) / 2;
-  const int64_t tasks = int64_t(p.m_tiles) * 32 * chunks;
-  const int64_t warps = int64_t(gridDim.x) * (kMxThreads / 32);
-  for (int64_t task = int64_t(blockIdx.x) * (kMxThreads / 32) + (threadIdx.x >> 5); task < tasks; task += warps) {
-    const int chunk = int(task % chunks);
-    const int64_t rows = task / chunks;
-    const int r = int(rows & 31), mt = int(rows >> 5);
+  const uint32_t tasks = uint32_t(p.m_tiles) * 32u * uint32_t(chunks), warps = gridDim.x * (kMxThreads / 32);
+  for (uint32_t task = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); task < tasks; task += warps) {
+    const int rows = int(task / uint32_t(chunks)), chunk = int(task) - rows * chunks;
+    const int r = rows & 31, mt = rows >> 5;
     const int col = chunk * 256 + lane * 8;
     if (col >= p.K) continue;
     const int kt = col >> 7, shift = 8 * ((lane >> 2) & 3);
