@@ -31,12 +31,11 @@ int check_codes(const void* q, int64_t ldq, const void* s, int M, int K) {
   return BFP8_OK;
 }
 
-int launch_mx(const void* kernel, int m_tiles, int k_tiles, void** args, int num_sms, cudaStream_t stream,
-              const char* what) {
+int launch_mx(const void* kernel, int m_tiles, int k_tiles, void** args, cudaStream_t stream, const char* what) {
   const int64_t tasks = int64_t(m_tiles) * 32 * cdiv(k_tiles, 2);
   if (tasks > INT32_MAX) return fail(BFP8_EINVAL, "too many rows x columns for one launch");
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(std::min<int64_t>((tasks + kMxThreads / 32 - 1) / (kMxThreads / 32), int64_t(num_sms) * 16)));
+  cfg.gridDim = dim3(unsigned((tasks + kMxThreads / 32 - 1) / (kMxThreads / 32)));
   cfg.blockDim = dim3(kMxThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -247,9 +246,9 @@ int moe_maps(MoeParams& mp, const MoeLayout& lay, int format, const void* w, int
     if (r != CUDA_SUCCESS) return fail(BFP8_ECUDA, "cuTensorMapEncodeTiled failed (" + std::to_string(int(r)) + ")");
     return int(BFP8_OK);
   };
-  // A short last column may be read past a row's end where another row of the
-  // stack follows in memory.
-  mp.tail_reads_on = bytes % 128 != 0 && w_expert >= w_row * rows;
+  // A short last column may be read past a row's end: another row of the stack
+  // follows in memory, but for the last one.
+  mp.tail_reads_on = bytes % 128 != 0;
   const uint64_t columns = full + (mp.tail_reads_on ? 1 : 0);
   if (columns > 0) {  // [128 bytes][rows][columns][halves][experts]
     const cuuint64_t dims[5] = {128, cuuint64_t(rows - half), columns, 2, cuuint64_t(E)};
@@ -298,6 +297,8 @@ int check_moe(const bfp8_moe_problem& p) {
   if (!aligned16(p.w13) || !aligned16(p.w2) || p.w13_row < k13 || p.w13_row % 16 || p.w2_row < k2 || p.w2_row % 16 ||
       p.w13_expert % 16 || p.w2_expert % 16)
     return fail(BFP8_EINVAL, "expert weights must be row-major with 16-byte aligned rows");
+  if (p.E > 1 && (p.w13_expert < 2 * p.I * p.w13_row || p.w2_expert < p.H * p.w2_row))
+    return fail(BFP8_EINVAL, "experts must not overlap or interleave");
   if (!aligned16(p.s13) || !aligned16(p.s2)) return fail(BFP8_EINVAL, "scales must be 16-byte aligned");
   return BFP8_OK;
 }
@@ -364,16 +365,13 @@ int bfp8_launch_mxfp4_quantize(const bfp8_mxfp4_quant_problem* pp, void* stream)
   if (p.M == 0) return BFP8_OK;
   if (!p.x || !aligned16(p.x) || p.ldx < p.K || (p.ldx * element_size(p.x_type)) % 16)
     return fail(BFP8_EINVAL, "x must be row-major with 16-byte aligned rows");
-  int dev = 0;
-  const int num_sms = current_device_sms(&dev);
-  if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");
   Mxfp4QuantParams k{p.x, p.ldx, static_cast<uint8_t*>(p.q), p.ldq, static_cast<uint8_t*>(p.s), p.M, p.K,
                      cdiv(p.M, 128), cdiv(p.K, 128), p.trigger ? 1 : 0};
   void* args[] = {&k};
   const void* kernel = p.x_type == 0   ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<float>)
                        : p.x_type == 1 ? reinterpret_cast<const void*>(&mxfp4_quantize_kernel<__nv_bfloat16>)
                                        : reinterpret_cast<const void*>(&mxfp4_quantize_kernel<__half>);
-  return launch_mx(kernel, k.m_tiles, k.k_tiles, args, num_sms, static_cast<cudaStream_t>(stream),
+  return launch_mx(kernel, k.m_tiles, k.k_tiles, args, static_cast<cudaStream_t>(stream),
                    "MXFP4 quantization launch");
 }
 
@@ -385,15 +383,12 @@ int bfp8_launch_mxfp4_dequantize(const bfp8_mxfp4_dequant_problem* pp, void* str
   if (p.M == 0) return BFP8_OK;
   if (!p.y || !aligned16(p.y) || p.ldy < p.K || (p.ldy * element_size(p.y_type)) % 16)
     return fail(BFP8_EINVAL, "y must be row-major with 16-byte aligned rows");
-  int dev = 0;
-  const int num_sms = current_device_sms(&dev);
-  if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");
   Mxfp4DequantParams k{static_cast<const uint8_t*>(p.q), p.ldq, static_cast<const uint8_t*>(p.s), p.y, p.ldy, p.M, p.K,
                        cdiv(p.M, 128), cdiv(p.K, 128)};
   void* args[] = {&k};
   const void* kernel = p.y_type == 0 ? reinterpret_cast<const void*>(&mxfp4_dequantize_kernel<float>)
                                      : reinterpret_cast<const void*>(&mxfp4_dequantize_kernel<__nv_bfloat16>);
-  return launch_mx(kernel, k.m_tiles, k.k_tiles, args, num_sms, static_cast<cudaStream_t>(stream),
+  return launch_mx(kernel, k.m_tiles, k.k_tiles, args, static_cast<cudaStream_t>(stream),
                    "MXFP4 dequantization launch");
 }
 

@@ -11,6 +11,14 @@
 // these sizes the weights of the chosen experts are the only traffic that
 // counts, so the kernels are built to stream them:
 //
+// Measured (B200, device time of a call in a graph): 64 tokens, 128 experts, top
+// 8, H = 4096, I = 1280 in block FP8: 342 us for 2.0 GB of weights, 0.9 of the
+// measured copy rate; 13 tokens, 64 experts, top 6, I = 1408: 131 us; one token,
+// 128 experts, top 8, H = 2048, I = 768: 26 us for 38 MB (6 us at that rate):
+// there the router (3 us), the hand-over between the kernels and their ends
+// count, not the stream.  MXFP4, 40 tokens, 64 experts, top 4, I = 2048: 170 us
+// for 0.8 GB.
+//
 // - Work: (token, expert) pairs are grouped by expert into chunks of up to
 //   8 NT tokens, in token order.  A unit is 16 weight rows (GATE: 8 gate rows
 //   and the 8 up rows beside them, so that one thread ends with both) of one
@@ -745,50 +753,48 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
 #pragma unroll
       for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
       for (int b0 = 0; b0 < unit_stages * stage_blocks; b0 += stage_blocks) {
-        {
-          const int s = group * ring + slot;
-          ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
-          const int nb = min(stage_blocks, blocks - b0);
-          const uint32_t stage = base + uint32_t(s) * stage_bytes;
-          // One 128-wide K block: its scales of rows g and g + 8, this lane's
-          // ldmatrix row (lanes 0-7 / 8-15 the two halves' rows in one 16-byte
-          // chunk, lanes 16-31 in the next), its token fragments and scales.
-          auto block = [&](int i, auto full_tag, int steps) {
-            constexpr bool FULL = decltype(full_tag)::value;
-            const int b = b0 + i;
-            float fa[4], fb[4];
-            if constexpr (MX) {
-              const uint32_t word = stage + 2u * half_bytes + uint32_t(i * 128 + g * 16);
-              e8m0x4_to_float(ld_shared_u32(word + word_a), fa);
-              e8m0x4_to_float(ld_shared_u32(word + word_b), fb);
-            } else {
-              fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][1], b & 31);
-              fb[0] = GATE ? __shfl_sync(~0u, b < 32 ? sc[1][0] : sc[1][1], b & 31) : fa[0];
-            }
-            const uint32_t a_row = stage + a_lane + uint32_t(MX ? i >> 1 : i) * 1024u;
-            const uint32_t chunk0 = (MX ? (i & 1) * 4u : 0u) + (lane >> 4);
-            uint32_t b_addr[NT];
+        const int s = group * ring + slot;
+        ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
+        const int nb = min(stage_blocks, blocks - b0);
+        const uint32_t stage = base + uint32_t(s) * stage_bytes;
+        // One 128-wide K block: its scales of rows g and g + 8, this lane's
+        // ldmatrix row (lanes 0-7 / 8-15 the two halves' rows in one 16-byte
+        // chunk, lanes 16-31 in the next), its token fragments and scales.
+        auto block = [&](int i, auto full_tag, int steps) {
+          constexpr bool FULL = decltype(full_tag)::value;
+          const int b = b0 + i;
+          float fa[4], fb[4];
+          if constexpr (MX) {
+            const uint32_t word = stage + 2u * half_bytes + uint32_t(i * 128 + g * 16);
+            e8m0x4_to_float(ld_shared_u32(word + word_a), fa);
+            e8m0x4_to_float(ld_shared_u32(word + word_b), fb);
+          } else {
+            fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][1], b & 31);
+            fb[0] = GATE ? __shfl_sync(~0u, b < 32 ? sc[1][0] : sc[1][1], b & 31) : fa[0];
+          }
+          const uint32_t a_row = stage + a_lane + uint32_t(MX ? i >> 1 : i) * 1024u;
+          const uint32_t chunk0 = (MX ? (i & 1) * 4u : 0u) + (lane >> 4);
+          uint32_t b_addr[NT];
 #pragma unroll
-            for (int c = 0; c < NT; ++c) b_addr[c] = b_lane[c] + uint32_t(b * 4) * piece;
-            const float* tsb = ts + b * 8 * NT + 2 * t4;
-            if (NT == 1 || count <= 8) moe_block<Cfg, 1, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
-            else moe_block<Cfg, NT, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
-          };
-          // Whole blocks two at a time (their loads and MMA chains overlap),
-          // then what is left; the last block of K may be short.
-          const int whole = min(nb, (k_len - b0 * 128) / 128);
-          int i = warp_in_group;
-          for (; i + kStep < whole; i += 2 * kStep) {
-            block(i, std::true_type(), 4);
-            block(i + kStep, std::true_type(), 4);
-          }
-          for (; i < nb; i += kStep) {
-            if (i < whole) block(i, std::true_type(), 4);
-            else block(i, std::false_type(), (k_len - (b0 + i) * 128) / 32);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(empty(s));
+          for (int c = 0; c < NT; ++c) b_addr[c] = b_lane[c] + uint32_t(b * 4) * piece;
+          const float* tsb = ts + b * 8 * NT + 2 * t4;
+          if (NT == 1 || count <= 8) moe_block<Cfg, 1, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
+          else moe_block<Cfg, NT, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
+        };
+        // Whole blocks two at a time (their loads and MMA chains overlap),
+        // then what is left; the last block of K may be short.
+        const int whole = min(nb, (k_len - b0 * 128) / 128);
+        int i = warp_in_group;
+        for (; i + kStep < whole; i += 2 * kStep) {
+          block(i, std::true_type(), 4);
+          block(i + kStep, std::true_type(), 4);
         }
+        for (; i < nb; i += kStep) {
+          if (i < whole) block(i, std::true_type(), 4);
+          else block(i, std::false_type(), (k_len - (b0 + i) * 128) / 32);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
         if (++slot == ring) slot = 0, phase ^= 1u;
       }
       // ---- this warp's sums of the unit
@@ -813,48 +819,48 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
     bool ok = true;
     for (; w.u < u1 && ok; next(w)) {
 #pragma unroll
-     for (int group = 0; group < G; ++group) {
-      if (group >= w.count) break;
-      const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
-      const int buf = int(done[group] % RB);
-      if (!(ok = mbar_wait(red_full(group, buf), done[group] / RB & 1u, abort_flag, kMoeWaitRedFull))) break;
-      ++done[group];
-      const int count = route.chunk_count[chunk];
-      const short* pairs = route.list + route.chunk_first[chunk];
+      for (int group = 0; group < G; ++group) {
+        if (group >= w.count) break;
+        const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
+        const int buf = int(done[group] % RB);
+        if (!(ok = mbar_wait(red_full(group, buf), done[group] / RB & 1u, abort_flag, kMoeWaitRedFull))) break;
+        ++done[group];
+        const int count = route.chunk_count[chunk];
+        const short* pairs = route.list + route.chunk_first[chunk];
 #pragma unroll
-      for (int c = 0; c < NT; ++c) {
-        if (c > 0 && c * 8 >= (p.resident ? p.cols : count)) break;
-        const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + ((buf * W + group * Cfg::GROUP_WARPS) * NT + c) * 32 + lane;
-        float4 v = red[0];
+        for (int c = 0; c < NT; ++c) {
+          if (c > 0 && c * 8 >= (p.resident ? p.cols : count)) break;
+          const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + ((buf * W + group * Cfg::GROUP_WARPS) * NT + c) * 32 + lane;
+          float4 v = red[0];
 #pragma unroll
-        for (int j = 1; j < Cfg::GROUP_WARPS; ++j) {
-          const float4 a = red[j * NT * 32];
-          v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
-        }
-        auto store = [&](int pair, float a, float b) {  // row g of either half
-          if constexpr (GATE) {
-            p.h[int64_t(pair) * p.I + tile * 8 + g] = a / (1.f + expf(-a)) * b;
+          for (int j = 1; j < Cfg::GROUP_WARPS; ++j) {
+            const float4 a = red[j * NT * 32];
+            v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+          }
+          auto store = [&](int pair, float a, float b) {  // row g of either half
+            if constexpr (GATE) {
+              p.h[int64_t(pair) * p.I + tile * 8 + g] = a / (1.f + expf(-a)) * b;
+            } else {
+              float* z = p.z + (int64_t(pair) * p.segments + seg) * p.H + tile * 16 + g;
+              z[0] = a;
+              z[8] = b;
+            }
+          };
+          // this lane has columns c 8 + 2 t4 and the next
+          if (p.resident) {
+            for (int k = 0; k < count; ++k) {
+              const int col = (GATE ? pairs[k] / p.top_k : pairs[k]) - c * 8;
+              if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);
+            }
           } else {
-            float* z = p.z + (int64_t(pair) * p.segments + seg) * p.H + tile * 16 + g;
-            z[0] = a;
-            z[8] = b;
+            const int col = c * 8 + 2 * t4;
+            if (col < count) store(pairs[col], v.x, v.z);
+            if (col + 1 < count) store(pairs[col + 1], v.y, v.w);
           }
-        };
-        // this lane has columns c 8 + 2 t4 and the next
-        if (p.resident) {
-          for (int k = 0; k < count; ++k) {
-            const int col = (GATE ? pairs[k] / p.top_k : pairs[k]) - c * 8;
-            if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);
-          }
-        } else {
-          const int col = c * 8 + 2 * t4;
-          if (col < count) store(pairs[col], v.x, v.z);
-          if (col + 1 < count) store(pairs[col + 1], v.y, v.w);
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(red_empty(group, buf));
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(red_empty(group, buf));
-     }
     }
   }
 }

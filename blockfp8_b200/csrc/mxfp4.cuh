@@ -115,7 +115,9 @@ constexpr int kMxThreads = 256;
 // A warp takes rows r, r + 32, r + 64, r + 96 of a 128-row tile over 256
 // columns: lane l holds values 8 l .. 8 l + 7 of each, a block is four lanes,
 // and the four rows' scale bytes of a K tile are 16 contiguous bytes.  Bound
-// by HBM; four independent loads per lane keep it fed.
+// by HBM; four independent loads per lane keep it fed.  24576 x 4096 bf16: 54 us
+// (4.7 TB/s), and 39 us (6.5 TB/s) back.  A warp a task: a grid of resident CTAs
+// that loop took 3 us longer for the two.
 template <class T>
 __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4QuantParams p) {
   // The wait comes first: a dependent that has started may then read whatever
@@ -126,8 +128,9 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_quantize_kernel(const Mxfp4Q
   if (p.trigger) griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int chunks = (p.k_tiles + 1) / 2;
-  const uint32_t tasks = uint32_t(p.m_tiles) * 32u * uint32_t(chunks), warps = gridDim.x * (kMxThreads / 32);
-  for (uint32_t task = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); task < tasks; task += warps) {
+  const uint32_t tasks = uint32_t(p.m_tiles) * 32u * uint32_t(chunks);
+  const uint32_t task = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5);
+  if (task < tasks) {
     const int rows = int(task / uint32_t(chunks)), chunk = int(task) - rows * chunks;  // (row tile, r)
     const int r = rows & 31, mt = rows >> 5;
     const int col = chunk * 256 + lane * 8;
@@ -185,12 +188,13 @@ __global__ void __launch_bounds__(kMxThreads) mxfp4_dequantize_kernel(const Mxfp
   griddep_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int chunks = (p.k_tiles + 1) / 2;
-  const uint32_t tasks = uint32_t(p.m_tiles) * 32u * uint32_t(chunks), warps = gridDim.x * (kMxThreads / 32);
-  for (uint32_t task = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); task < tasks; task += warps) {
+  const uint32_t tasks = uint32_t(p.m_tiles) * 32u * uint32_t(chunks);
+  const uint32_t task = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5);
+  if (task < tasks) {
     const int rows = int(task / uint32_t(chunks)), chunk = int(task) - rows * chunks;
     const int r = rows & 31, mt = rows >> 5;
     const int col = chunk * 256 + lane * 8;
-    if (col >= p.K) continue;
+    if (col >= p.K) return;
     const int kt = col >> 7, shift = 8 * ((lane >> 2) & 3);
     const uint4 words = *reinterpret_cast<const uint4*>(p.s + ((int64_t(mt) * p.k_tiles + kt) * 32 + r) * 16);
     const uint32_t word[4] = {words.x, words.y, words.z, words.w};

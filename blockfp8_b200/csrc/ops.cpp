@@ -487,6 +487,8 @@ void check_experts(const at::Tensor& w, const at::Tensor& s, int64_t E, int64_t 
   const int64_t cols = mx ? K / 2 : K;
   CHECK_VALUE(w.dim() == 3 && w.size(0) == E && w.size(1) == rows && w.size(2) == cols, op, ": ", name, " must be [", E, ", ", rows, ", ",
               cols, "], got ", w.sizes());
+  CHECK_VALUE(E == 1 || w.stride(0) >= rows * w.stride(1), op, ": the experts of ", name,
+              " must not overlap or interleave, got strides ", w.strides());
   CHECK_VALUE(w.stride(2) == 1 && w.stride(1) >= cols && w.stride(1) % 16 == 0 && w.stride(0) % 16 == 0 && aligned16(w),
               op, ": ", name, " must have contiguous, 16-byte aligned rows, got strides ", w.strides());
   if (mx) {

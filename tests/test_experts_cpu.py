@@ -118,6 +118,7 @@ def _moe(t=3, h=64, e=4, top_k=2, layer=None, x=None, logits=None):
     (lambda: _moe(layer=_layer()[:2] + _layer(fmt="mxfp4")[2:]), "w13 and w2|w2 must be|w13 must be"),
     (lambda: _moe(layer=[_layer()[0], _layer()[1][:, :1], *_layer()[2:]]), "scales of w13"),
     (lambda: _moe(layer=[*_layer()[:3], _layer()[3].double()]), "scales of w2"),
+    (lambda: _moe(layer=[_layer()[0][:1].expand(4, -1, -1), *_layer()[1:]]), "overlap"),
     (lambda: _moe(layer=[_layer()[0].transpose(1, 2).contiguous().transpose(1, 2), *_layer()[1:]]), "rows"),
 ])
 def test_moe_refusals(call, reason):
@@ -181,7 +182,7 @@ def test_every_allowed_layer_has_a_layout(fmt):
     """Shared memory holds some layout of every size that the checks let through."""
     lib = _native.capi()
     m = _native.MoeProblem(x=16, ldx=8192, x_type=1, logits=16, ld_logits=512, logits_type=0, format=fmt, w13=16,
-                           w13_expert=16, w13_row=1 << 20, s13=16, w2=16, w2_expert=16, w2_row=1 << 20, s2=16, y=16, ldy=8192)
+                           w13_expert=1 << 36, w13_row=1 << 15, s13=16, w2=16, w2_expert=1 << 36, w2_row=1 << 15, s2=16, y=16, ldy=8192)
     for m.T in (1, 2, 7, 8, 9, 16, 17, 33, 64):
         for m.H in (32, 96, 1024, 2880, 4096, 4128, 7168, 8160, 8192):
             for m.I in (32, 128, 1408, 2880, 4096, 4128, 14336, 16384 + 32):

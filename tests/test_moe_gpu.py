@@ -157,6 +157,12 @@ def test_ties_and_masked_logits():
         assert (y[2] == 0).all()
 
 
+def test_no_tokens():
+    layer = Layer("fp8", 4, 64, 32, seed=1)
+    x = torch.empty(0, 64, dtype=torch.bfloat16, device=DEV)
+    assert bf.moe(x, torch.empty(0, 4, device=DEV), *layer.args, top_k=2).shape == (0, 64)
+
+
 def test_values_far_apart():
     # activations over the whole of bf16's range beside ordinary ones
     layer = Layer("mxfp4", 4, 256, 128, seed=15)
