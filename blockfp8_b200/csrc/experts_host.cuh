@@ -167,7 +167,7 @@ struct MoeLayout {
 // K of `k` values in `segments` ranges, `entries` tokens or pairs that could
 // have a column of their own, in stages of up to max_box 128-byte columns and
 // within `limit` bytes of shared memory.
-bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int nt, int warps, int max_box, int limit,
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int warps, int max_box, int limit,
                 MoeLayout* out) {
   const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
   const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, max_box);
@@ -175,17 +175,16 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
   out->unit_stages = unit_stages;
   out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
   out->segments = cdiv(k, out->seg_len);
-  out->resident = entries <= 8 * nt;
-  out->cols = out->resident ? entries : std::min(P, 8 * nt);
+  out->resident = entries <= kMoeChunk;
+  out->cols = out->resident ? entries : std::min(P, kMoeChunk);
   const int blocks = cdiv(std::min(k, out->seg_len), 128);
   const int stage = round_up(out->box * (2048 + (p.format ? 512 : 0)), 1024);
-  const int red_bufs = warps * nt >= 32 ? 1 : 2;
-  const int b = blocks * 256 * out->cols, ts = round_up(blocks * 8 * nt * 4, 16);
-  const int red = red_bufs * warps * nt * 512, route = round_up(moe_route_bytes(P), 16);
+  const int b = blocks * 256 * out->cols, ts = blocks * kMoeChunk * 4;
+  const int red = kMoeRedBufs * warps * 512, route = round_up(moe_route_bytes(P), 16);
   const int scratch = P > 32 ? p.E * (cdiv(P, 32) + 1) * 4 : 0;
-  auto end_of = [&](int stages) { return 8 * (2 * stages + 2 * warps / moe_group_warps(warps, nt) * red_bufs) + 16 + 4 * stages; };
+  auto end_of = [&](int stages) { return 8 * (2 * stages + 2 * warps / kMoeGroupWarps * kMoeRedBufs) + 16 + 4 * stages; };
   const int fixed = 1024 + b + ts + red + route + end_of(16);
-  const int groups = warps / moe_group_warps(warps, nt);
+  const int groups = warps / kMoeGroupWarps;
   const int stages = std::min(16, (limit - fixed) / stage) / groups * groups;
   if (stages < 2 * groups) return false;
   // the routing scratch lies where the ring and, unless they come first, the activations do
@@ -202,29 +201,24 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
 }
 
 struct MoeShape {
-  int nt, warps;  // 8-token tiles of a chunk; consumer warps
+  int warps;  // consumers
   MoeLayout gate, down;
 };
 
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
   const int P = p.T * p.top_k, segments = cdiv(p.I, kMoeSegment);
-  auto fits = [&](int nt, int warps, int limit) {
-    s->nt = nt;
+  auto fits = [&](int warps, int limit) {
     s->warps = warps;
     auto one = [&](int k, int ranges, int entries, MoeLayout* lay) {
       for (int box = 8; box >= 1; box /= 2)
-        if (moe_layout(p, k, ranges, entries, nt, warps, box, limit, lay)) return true;
+        if (moe_layout(p, k, ranges, entries, warps, box, limit, lay)) return true;
       return false;
     };
     return one(p.H, 1, p.T, &s->gate) && one(p.I, segments, P, &s->down);
   };
   // Up to 8 tokens: both kernels in half an SM's shared memory, so that DOWN
   // starts beside GATE and requests its weights while GATE runs.
-  if (p.T <= 8 && fits(1, 8, kMoeHalfSmem)) return true;
-  // Chunks of 16 where experts have more than four tokens on average, else of
-  // 8: a ring twice as deep, and few experts are read twice.
-  if (p.T > 8 && P > 4 * p.E && fits(2, 16, kMaxSmem)) return true;
-  return fits(1, 16, kMaxSmem);
+  return (p.T <= 8 && fits(8, kMoeHalfSmem)) || fits(16, kMaxSmem);
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
@@ -335,19 +329,15 @@ int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms,
 template <bool GATE>
 int launch_moe_any(MoeParams& mp, const MoeLayout& lay, int format, const MoeShape& s, int x_type, int dev, int num_sms,
                    cudaStream_t stream) {
-  auto go = [&](auto mx, auto tiles, auto warps, auto t) {
-    return launch_moe_kernel<MoeCfg<GATE, decltype(mx)::value, decltype(tiles)::value, decltype(warps)::value, decltype(t)>>(
-        mp, lay, dev, num_sms, stream);
+  auto go = [&](auto mx, auto warps, auto t) {
+    return launch_moe_kernel<MoeCfg<GATE, decltype(mx)::value, decltype(warps)::value, decltype(t)>>(mp, lay, dev, num_sms,
+                                                                                                   stream);
   };
-  using One = std::integral_constant<int, 1>;
-  using Two = std::integral_constant<int, 2>;
-  using W8 = std::integral_constant<int, 8>;
-  using W16 = std::integral_constant<int, 16>;
-  auto by_type = [&](auto mx, auto tiles, auto warps) {
-    return x_type == 1 ? go(mx, tiles, warps, __nv_bfloat16()) : go(mx, tiles, warps, __half());
+  auto by_type = [&](auto mx, auto warps) {
+    return x_type == 1 ? go(mx, warps, __nv_bfloat16()) : go(mx, warps, __half());
   };
   auto by_shape = [&](auto mx) {
-    return s.nt == 2 ? by_type(mx, Two(), W16()) : s.warps == 16 ? by_type(mx, One(), W16()) : by_type(mx, One(), W8());
+    return s.warps == 16 ? by_type(mx, std::integral_constant<int, 16>()) : by_type(mx, std::integral_constant<int, 8>());
   };
   return format ? by_shape(std::true_type()) : by_shape(std::false_type());
 }

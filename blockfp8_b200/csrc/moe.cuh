@@ -20,7 +20,9 @@
 // for 0.8 GB.
 //
 // - Work: (token, expert) pairs are grouped by expert into chunks of up to
-//   8 NT tokens, in token order.  A unit is 16 weight rows (GATE: 8 gate rows
+//   8, in token order (busier experts are read again, mostly from L2: chunks of 16
+//   with two MMA tiles and half the ring took 1.4 to 2.2 times as long for 5 to
+//   25 tokens an expert).  A unit is 16 weight rows (GATE: 8 gate rows
 //   and the 8 up rows beside them, so that one thread ends with both) of one
 //   chunk over a whole K range, and CTA b of G takes units [U b / G, U (b+1) / G).
 //   16 rows keep the last wave short (one token, 8 experts of I = 768: 768
@@ -391,42 +393,34 @@ __global__ void __launch_bounds__(kMoeSumThreads) moe_sum_kernel(const MoeSumPar
   *reinterpret_cast<uint2*>(static_cast<T*>(p.y) + int64_t(t) * p.ldy + col) = out;
 }
 
-// Consumer warps work in groups, each on a unit of its own.  16 tokens a chunk
-// leave little room for rings: two groups of eight then.
-constexpr int moe_group_warps(int warps, int nt) { return nt == 2 ? warps / 2 : 4; }
+constexpr int kMoeChunk = 8;       // most pairs of a chunk: the MMA's columns
+constexpr int kMoeGroupWarps = 4;  // consumer warps of a group, which works on a unit of its own
+constexpr int kMoeRedBufs = 2;     // buffers of the warps' sums (512 bytes a warp)
 
-template <bool GATE_, bool MX_, int NT_, int WARPS_, class T_>
+template <bool GATE_, bool MX_, int WARPS_, class T_>
 struct MoeCfg {
   static constexpr bool GATE = GATE_, MX = MX_;
-  static constexpr int NT = NT_;        // 8-token MMA tiles of a chunk
   static constexpr int WARPS = WARPS_;  // consumers
-  static constexpr int GROUP_WARPS = moe_group_warps(WARPS, NT);
-  static constexpr int GROUPS = WARPS / GROUP_WARPS;
+  static constexpr int GROUPS = WARPS / kMoeGroupWarps;
   static constexpr int PRODUCERS = WARPS == 16 ? 2 : 1;
   static constexpr int THREADS = 32 * (WARPS + PRODUCERS + 1);
-  static constexpr int RED_BUFS = WARPS * NT >= 32 ? 1 : 2;  // buffers of the warps' sums (512 NT bytes a warp)
   static constexpr int CTAS_PER_SM = WARPS == 8 ? 2 : 1;
   using T = T_;                   // x and y
   static constexpr int BLOCK_BYTES = MX ? 64 : 128;  // 128 values of K of one row
 };
 
-// acc += one 128-wide K block of 16 weight rows times the chunk's tokens (C
-// tiles of 8).  a_row, chunk0: this lane's ldmatrix row and first 16-byte chunk
-// in it; b_addr: its piece of the tokens' fragments per tile, piece bytes apart
-// per 32 values of K.
-// FULL: all four 32-wide steps, so that every load can go out first; else
-// `steps` of them.
-template <class Cfg, int C, bool FULL>
-__device__ __forceinline__ void moe_block(float (&acc)[Cfg::NT][4], uint32_t a_row, uint32_t chunk0,
-                                          const uint32_t (&b_addr)[Cfg::NT], uint32_t piece, int steps, const float (&fa)[4], const float (&fb)[4],
+// acc += one 128-wide K block of 16 weight rows times the chunk's 8 tokens.
+// a_row, chunk0: this lane's ldmatrix row and first 16-byte chunk in it;
+// b_addr: its piece of the tokens' fragments, piece bytes apart per 32 values
+// of K.  FULL: all four 32-wide steps, so that every load can go out first;
+// else `steps` of them.
+template <class Cfg, bool FULL>
+__device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint32_t chunk0, uint32_t b_addr,
+                                          uint32_t piece, int steps, const float (&fa)[4], const float (&fb)[4],
                                           const float* ts) {
   // the 128-byte swizzle: chunk XOR row inside 8 rows
   auto chunk_at = [&](uint32_t c) { return a_row + (((chunk0 + c) ^ (threadIdx.x & 7u)) << 4); };
-  float part[C][2][4];
-#pragma unroll
-  for (int c = 0; c < C; ++c)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) part[c][h][0] = part[c][h][1] = part[c][h][2] = part[c][h][3] = 0.f;
+  float part[2][4] = {};
   if constexpr (Cfg::MX) {
     uint32_t r[4][2];  // [step][8-row half]: eight codes
 #pragma unroll
@@ -442,18 +436,15 @@ __device__ __forceinline__ void moe_block(float (&acc)[Cfg::NT][4], uint32_t a_r
         uint32_t ha[4], hb[4];
         e2m1x8_to_f16(r[s][0], ha);
         e2m1x8_to_f16(r[s][1], hb);
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const uint4 b = ld_shared_v4(b_addr[c] + uint32_t(s) * piece);
-          float d[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(d, ha[0], hb[0], ha[1], hb[1], b.x, b.y);
-          mma_f16(d, ha[2], hb[2], ha[3], hb[3], b.z, b.w);
-          float(&q)[4] = part[c][s & 1];
-          q[0] = fmaf(d[0], fa[s], q[0]);
-          q[1] = fmaf(d[1], fa[s], q[1]);
-          q[2] = fmaf(d[2], fb[s], q[2]);
-          q[3] = fmaf(d[3], fb[s], q[3]);
-        }
+        const uint4 b = ld_shared_v4(b_addr + uint32_t(s) * piece);
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma_f16(d, ha[0], hb[0], ha[1], hb[1], b.x, b.y);
+        mma_f16(d, ha[2], hb[2], ha[3], hb[3], b.z, b.w);
+        float(&q)[4] = part[s & 1];
+        q[0] = fmaf(d[0], fa[s], q[0]);
+        q[1] = fmaf(d[1], fa[s], q[1]);
+        q[2] = fmaf(d[2], fb[s], q[2]);
+        q[3] = fmaf(d[3], fb[s], q[3]);
       }
   } else {
     uint32_t r[4][4];
@@ -466,29 +457,23 @@ __device__ __forceinline__ void moe_block(float (&acc)[Cfg::NT][4], uint32_t a_r
         uint32_t lo[4], hi[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) e4m3x4_to_f16(r[s][k], lo[k], hi[k]);
-#pragma unroll
-        for (int c = 0; c < C; ++c) {
-          const uint4 b = ld_shared_v4(b_addr[c] + uint32_t(s) * piece);
-          mma_f16(part[c][0], lo[0], lo[1], hi[0], hi[1], b.x, b.y);
-          mma_f16(part[c][1], lo[2], lo[3], hi[2], hi[3], b.z, b.w);
-        }
+        const uint4 b = ld_shared_v4(b_addr + uint32_t(s) * piece);
+        mma_f16(part[0], lo[0], lo[1], hi[0], hi[1], b.x, b.y);
+        mma_f16(part[1], lo[2], lo[3], hi[2], hi[3], b.z, b.w);
       }
   }
   const float sa = Cfg::MX ? 1.f : fa[0], sb = Cfg::MX ? 1.f : fb[0];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const float2 t = *reinterpret_cast<const float2*>(ts + c * 8);
-    acc[c][0] = fmaf(part[c][0][0] + part[c][1][0], t.x * sa, acc[c][0]);
-    acc[c][1] = fmaf(part[c][0][1] + part[c][1][1], t.y * sa, acc[c][1]);
-    acc[c][2] = fmaf(part[c][0][2] + part[c][1][2], t.x * sb, acc[c][2]);
-    acc[c][3] = fmaf(part[c][0][3] + part[c][1][3], t.y * sb, acc[c][3]);
-  }
+  const float2 t = *reinterpret_cast<const float2*>(ts);
+  acc[0] = fmaf(part[0][0] + part[1][0], t.x * sa, acc[0]);
+  acc[1] = fmaf(part[0][1] + part[1][1], t.y * sa, acc[1]);
+  acc[2] = fmaf(part[0][2] + part[1][2], t.x * sb, acc[2]);
+  acc[3] = fmaf(part[0][3] + part[1][3], t.y * sb, acc[3]);
 }
 
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(const __grid_constant__ MoeParams p) {
   constexpr bool GATE = Cfg::GATE, MX = Cfg::MX;
-  constexpr int NT = Cfg::NT, BB = Cfg::BLOCK_BYTES, W = Cfg::WARPS, G = Cfg::GROUPS, RB = Cfg::RED_BUFS;
+  constexpr int BB = Cfg::BLOCK_BYTES, W = Cfg::WARPS, G = Cfg::GROUPS, RB = kMoeRedBufs;
   constexpr int THREADS = Cfg::THREADS, PRODUCERS = Cfg::PRODUCERS;
   using T = typename Cfg::T;
   extern __shared__ uint8_t smem_raw[];
@@ -513,11 +498,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
     for (int s = 0; s < S; ++s) {
       issued[s] = 0;
       mbar_init(full(s), 1u);
-      mbar_init(empty(s), Cfg::GROUP_WARPS);
+      mbar_init(empty(s), kMoeGroupWarps);
     }
     for (int g = 0; g < G; ++g)
       for (int b = 0; b < RB; ++b) {
-        mbar_init(red_full(g, b), Cfg::GROUP_WARPS);
+        mbar_init(red_full(g, b), kMoeGroupWarps);
         mbar_init(red_empty(g, b), 1u);
       }
     *abort_flag = 0;
@@ -532,7 +517,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   // two per column and 128-wide block.  A column past the batch reads some
   // other token's values and is not used.
   uint8_t* bfrag = smem + p.off_b;
-  float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8 NT]
+  float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8]
   const uint32_t piece = uint32_t(p.cols) * 64u;
   auto fragments = [&](int columns, int k_len, auto row_of) {  // by the consumer warps
     const int blocks = (k_len + 127) / 128, tasks = columns * blocks;
@@ -573,7 +558,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
             *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
             *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
           }
-          if (l16 == 0) ts[b * 8 * NT + col] = back;
+          if (l16 == 0) ts[b * kMoeChunk + col] = back;
         }
       }
     }
@@ -686,10 +671,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   } else if (warp < W) {
     // ---------------------------------------------------------------- consumers
     const int g = lane >> 2, t4 = lane & 3;
-    uint32_t b_lane[NT];
-#pragma unroll
-    for (int c = 0; c < NT; ++c) b_lane[c] = base + p.off_b + uint32_t(min(c * 8 + g, p.cols - 1) * 64 + t4 * 16);
-    constexpr int kStep = Cfg::GROUP_WARPS;
+    const uint32_t b_lane = base + p.off_b + uint32_t(min(g, p.cols - 1) * 64 + t4 * 16);
+    constexpr int kStep = kMoeGroupWarps;
     const int group = warp / kStep, warp_in_group = warp % kStep;
     const uint32_t a_lane = ((lane >> 3) & 1) * half_bytes + (lane & 7) * 128u;
     int have = -1, count = 0, done = 0, slot = 0;
@@ -749,9 +732,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
       // MXFP4: the 32-row quarter of the rows' scale tiles
       const uint32_t word_a = uint32_t(((GATE ? tile * 8 : tile * 16) >> 5) & 3) * 4u;
       const uint32_t word_b = scale_copy + uint32_t(((GATE ? p.I + tile * 8 : tile * 16 + 8) >> 5) & 3) * 4u;
-      float acc[NT][4];
-#pragma unroll
-      for (int i = 0; i < NT; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+      float acc[4] = {0.f, 0.f, 0.f, 0.f};
       for (int b0 = 0; b0 < unit_stages * stage_blocks; b0 += stage_blocks) {
         const int s = group * ring + slot;
         ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
@@ -774,12 +755,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
           }
           const uint32_t a_row = stage + a_lane + uint32_t(MX ? i >> 1 : i) * 1024u;
           const uint32_t chunk0 = (MX ? (i & 1) * 4u : 0u) + (lane >> 4);
-          uint32_t b_addr[NT];
-#pragma unroll
-          for (int c = 0; c < NT; ++c) b_addr[c] = b_lane[c] + uint32_t(b * 4) * piece;
-          const float* tsb = ts + b * 8 * NT + 2 * t4;
-          if (NT == 1 || count <= 8) moe_block<Cfg, 1, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
-          else moe_block<Cfg, NT, FULL>(acc, a_row, chunk0, b_addr, piece, steps, fa, fb, tsb);
+          moe_block<Cfg, FULL>(acc, a_row, chunk0, b_lane + uint32_t(b * 4) * piece, piece, steps, fa, fb,
+                               ts + b * kMoeChunk + 2 * t4);
         };
         // Whole blocks two at a time (their loads and MMA chains overlap),
         // then what is left; the last block of K may be short.
@@ -801,9 +778,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
       const int buf = done % RB;
       if (done >= RB) ok = mbar_wait(red_empty(group, buf), uint32_t(done / RB - 1) & 1u, abort_flag, kMoeWaitRedEmpty) && ok;
       ++done;
-      float4* red = reinterpret_cast<float4*>(smem + p.off_red) + (buf * W + warp) * NT * 32 + lane;
-#pragma unroll
-      for (int c = 0; c < NT; ++c) red[c * 32] = make_float4(acc[c][0], acc[c][1], acc[c][2], acc[c][3]);
+      reinterpret_cast<float4*>(smem + p.off_red)[(buf * W + warp) * 32 + lane] =
+          make_float4(acc[0], acc[1], acc[2], acc[3]);
       __syncwarp();
       if (lane == 0) mbar_arrive(red_full(group, buf));
     }
@@ -827,36 +803,32 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         ++done[group];
         const int count = route.chunk_count[chunk];
         const short* pairs = route.list + route.chunk_first[chunk];
+        const float4* red =
+            reinterpret_cast<const float4*>(smem + p.off_red) + (buf * W + group * kMoeGroupWarps) * 32 + lane;
+        float4 v = red[0];
 #pragma unroll
-        for (int c = 0; c < NT; ++c) {
-          if (c > 0 && c * 8 >= (p.resident ? p.cols : count)) break;
-          const float4* red = reinterpret_cast<const float4*>(smem + p.off_red) + ((buf * W + group * Cfg::GROUP_WARPS) * NT + c) * 32 + lane;
-          float4 v = red[0];
-#pragma unroll
-          for (int j = 1; j < Cfg::GROUP_WARPS; ++j) {
-            const float4 a = red[j * NT * 32];
-            v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
-          }
-          auto store = [&](int pair, float a, float b) {  // row g of either half
-            if constexpr (GATE) {
-              p.h[int64_t(pair) * p.I + tile * 8 + g] = a / (1.f + expf(-a)) * b;
-            } else {
-              float* z = p.z + (int64_t(pair) * p.segments + seg) * p.H + tile * 16 + g;
-              z[0] = a;
-              z[8] = b;
-            }
-          };
-          // this lane has columns c 8 + 2 t4 and the next
-          if (p.resident) {
-            for (int k = 0; k < count; ++k) {
-              const int col = (GATE ? pairs[k] / p.top_k : pairs[k]) - c * 8;
-              if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);
-            }
+        for (int j = 1; j < kMoeGroupWarps; ++j) {
+          const float4 a = red[j * 32];
+          v.x += a.x, v.y += a.y, v.z += a.z, v.w += a.w;
+        }
+        auto store = [&](int pair, float a, float b) {  // row g of either half
+          if constexpr (GATE) {
+            p.h[int64_t(pair) * p.I + tile * 8 + g] = a / (1.f + expf(-a)) * b;
           } else {
-            const int col = c * 8 + 2 * t4;
-            if (col < count) store(pairs[col], v.x, v.z);
-            if (col + 1 < count) store(pairs[col + 1], v.y, v.w);
+            float* z = p.z + (int64_t(pair) * p.segments + seg) * p.H + tile * 16 + g;
+            z[0] = a;
+            z[8] = b;
           }
+        };
+        // this lane has columns 2 t4 and the next
+        if (p.resident) {
+          for (int k = 0; k < count; ++k) {
+            const int col = GATE ? pairs[k] / p.top_k : pairs[k];
+            if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);
+          }
+        } else {
+          if (2 * t4 < count) store(pairs[2 * t4], v.x, v.z);
+          if (2 * t4 + 1 < count) store(pairs[2 * t4 + 1], v.y, v.w);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(red_empty(group, buf));
