@@ -155,19 +155,21 @@ int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaS
 
 constexpr int kMoeMaxHidden = 8192;
 constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
+constexpr int kMoeBusySegment = 2048;  // the same with eight columns: 64 KB, which leaves the ring its depth
 constexpr int kMoeHalfSmem = 113 * 1024;
+constexpr int kMoeSharedSmem = 226 * 1024;  // of two CTAs on an SM, without what the system takes
 
 // How one kernel's units (segments of seg_len values of K) and shared memory
 // are laid out.
 struct MoeLayout {
   int segments, seg_len, box, unit_stages, stages, smem, cols, resident;
-  uint32_t off_b, off_ts, off_red, off_route, off_bars;
+  uint32_t off_b, off_ts, off_red, off_route, off_bars, low;
 };
 
 // K of `k` values in `segments` ranges, `entries` tokens or pairs that could
-// have a column of their own, in stages of up to max_box 128-byte columns and
-// within `limit` bytes of shared memory.
-bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int warps, int max_box, int limit,
+// have a column of their own (in `parts` f16 parts), in stages of up to max_box
+// 128-byte columns and within `limit` bytes of shared memory.
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int parts, int warps, int max_box, int limit,
                 MoeLayout* out) {
   const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
   const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, max_box);
@@ -179,7 +181,7 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
   out->cols = out->resident ? entries : std::min(P, kMoeChunk);
   const int blocks = cdiv(std::min(k, out->seg_len), 128);
   const int stage = round_up(out->box * (2048 + (p.format ? 512 : 0)), 1024);
-  const int b = blocks * 256 * out->cols, ts = blocks * kMoeChunk * 4;
+  const int b = blocks * 256 * out->cols * parts, ts = blocks * kMoeChunk * 4;
   const int red = kMoeRedBufs * warps * 512, route = round_up(moe_route_bytes(P), 16);
   const int scratch = P > 32 ? p.E * (cdiv(P, 32) + 1) * 4 : 0;
   auto end_of = [&](int stages) { return 8 * (2 * stages + 2 * warps / kMoeGroupWarps * kMoeRedBufs) + 16 + 4 * stages; };
@@ -192,6 +194,7 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
   if (fixed + ring > limit) return false;
   out->stages = stages;
   out->off_b = uint32_t(ring);
+  out->low = uint32_t(b / parts);
   out->off_ts = out->off_b + uint32_t(b);
   out->off_red = out->off_ts + uint32_t(ts);
   out->off_route = out->off_red + uint32_t(red);
@@ -206,19 +209,20 @@ struct MoeShape {
 };
 
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
-  const int P = p.T * p.top_k, segments = cdiv(p.I, kMoeSegment);
-  auto fits = [&](int warps, int limit) {
+  const int P = p.T * p.top_k, segments = cdiv(p.I, P > kMoeChunk / 2 ? kMoeBusySegment : kMoeSegment);
+  auto one = [&](int k, int ranges, int entries, int parts, int warps, int limit, MoeLayout* lay) {
     s->warps = warps;
-    auto one = [&](int k, int ranges, int entries, MoeLayout* lay) {
-      for (int box = 8; box >= 1; box /= 2)
-        if (moe_layout(p, k, ranges, entries, warps, box, limit, lay)) return true;
-      return false;
-    };
-    return one(p.H, 1, p.T, &s->gate) && one(p.I, segments, P, &s->down);
+    for (int box = 8; box >= 1; box /= 2)
+      if (moe_layout(p, k, ranges, entries, parts, warps, box, limit, lay)) return true;
+    return false;
   };
-  // Up to 8 tokens: both kernels in half an SM's shared memory, so that DOWN
-  // starts beside GATE and requests its weights while GATE runs.
-  return (p.T <= 8 && fits(8, kMoeHalfSmem)) || fits(16, kMaxSmem);
+  // Up to 8 tokens: GATE in half an SM's shared memory and DOWN in what it
+  // leaves, so that DOWN starts beside GATE and requests its weights while GATE
+  // runs.
+  if (p.T <= 8 && one(p.H, 1, p.T, 1, 8, kMoeHalfSmem, &s->gate) &&
+      one(p.I, segments, P, 2, 8, kMoeSharedSmem - s->gate.smem, &s->down))
+    return true;
+  return one(p.H, 1, p.T, 1, 16, kMaxSmem, &s->gate) && one(p.I, segments, P, 2, 16, kMaxSmem, &s->down);
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
@@ -311,6 +315,7 @@ int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms,
   mp.off_red = lay.off_red;
   mp.off_route = lay.off_route;
   mp.off_bars = lay.off_bars;
+  mp.low = lay.low;
   mp.cols = lay.cols;
   mp.resident = lay.resident;
   cudaLaunchConfig_t cfg{};

@@ -42,8 +42,12 @@
 //   directly; tcgen05 would need them written back to shared memory.
 // - Activations are held in shared memory as f16 in MMA fragment order with
 //   one power-of-two scale per token and 128 values, which puts the largest
-//   at 2^14: bf16 values are exact down to 2^-28 of it, and h (fp32) keeps 11
-//   bits, 8 times finer than a bf16 h would.
+//   at 2^14: bf16 values are exact down to 2^-28 of it.  h (fp32) takes two
+//   f16 parts, the value rounded and what that leaves: 22 bits of each value,
+//   at worst 2^-39 of the largest.  Up to four pairs have their upper parts in
+//   the MMA's columns 0-3 and the lower ones in 4-7; more take a second pass over
+//   the stage.  (Both parts against the weights once converted: spills, and 1 us
+//   of 28 for one token, which needs no second pass.)
 // - A last warp finishes units: it adds the consumers' sums in warp order.
 //   z goes to memory and a small third kernel adds each token's pairs in j
 //   order.  (Counting arrivals and letting the last unit of an output row tile
@@ -98,6 +102,7 @@ struct MoeParams {
   int cols;               // token columns held
   int resident;           // every token (GATE) or pair (DOWN) has its own
   uint32_t off_b, off_ts, off_red, off_route, off_bars;  // shared memory
+  uint32_t low;  // DOWN: from h's upper parts to its lower ones
 };
 
 struct MoeSumParams {
@@ -352,6 +357,12 @@ __device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What rounding a and b to the f16 pair `upper` leaves (exact), as a pair.
+__device__ __forceinline__ uint32_t f16x2_rest(float a, float b, uint32_t upper) {
+  const float2 u = __half22float2(*reinterpret_cast<const __half2*>(&upper));
+  return pack_f16x2(a - u.x, b - u.y);
+}
+
 // 2^(14 - floor(log2 amax)), kept finite, and its inverse.
 __device__ __forceinline__ void moe_act_scale(uint32_t amax_bits, float& to, float& back) {
   const int e = int(amax_bits >> 23);  // biased; 0: zero or subnormal, 255: inf or NaN
@@ -394,6 +405,7 @@ __global__ void __launch_bounds__(kMoeSumThreads) moe_sum_kernel(const MoeSumPar
 }
 
 constexpr int kMoeChunk = 8;       // most pairs of a chunk: the MMA's columns
+constexpr int kMoeBeside = 4;      // most pairs whose h has both parts in one MMA's columns
 constexpr int kMoeGroupWarps = 4;  // consumer warps of a group, which works on a unit of its own
 constexpr int kMoeRedBufs = 2;     // buffers of the warps' sums (512 bytes a warp)
 
@@ -409,15 +421,15 @@ struct MoeCfg {
   static constexpr int BLOCK_BYTES = MX ? 64 : 128;  // 128 values of K of one row
 };
 
-// acc += one 128-wide K block of 16 weight rows times the chunk's 8 tokens.
+// acc += one 128-wide K block of 16 weight rows times the chunk's 8 columns.
 // a_row, chunk0: this lane's ldmatrix row and first 16-byte chunk in it;
 // b_addr: its piece of the tokens' fragments, piece bytes apart per 32 values
-// of K.  FULL: all four 32-wide steps, so that every load can go out first;
+// of K; ts0, ts1: the scales of this lane's two columns.  FULL: all four 32-wide steps, so that every load can go out first;
 // else `steps` of them.
 template <class Cfg, bool FULL>
 __device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint32_t chunk0, uint32_t b_addr,
-                                          uint32_t piece, int steps, const float (&fa)[4], const float (&fb)[4],
-                                          const float* ts) {
+                                          uint32_t piece, int steps, const float (&fa)[4],
+                                          const float (&fb)[4], float ts0, float ts1) {
   // the 128-byte swizzle: chunk XOR row inside 8 rows
   auto chunk_at = [&](uint32_t c) { return a_row + (((chunk0 + c) ^ (threadIdx.x & 7u)) << 4); };
   float part[2][4] = {};
@@ -463,11 +475,10 @@ __device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint3
       }
   }
   const float sa = Cfg::MX ? 1.f : fa[0], sb = Cfg::MX ? 1.f : fb[0];
-  const float2 t = *reinterpret_cast<const float2*>(ts);
-  acc[0] = fmaf(part[0][0] + part[1][0], t.x * sa, acc[0]);
-  acc[1] = fmaf(part[0][1] + part[1][1], t.y * sa, acc[1]);
-  acc[2] = fmaf(part[0][2] + part[1][2], t.x * sb, acc[2]);
-  acc[3] = fmaf(part[0][3] + part[1][3], t.y * sb, acc[3]);
+  acc[0] = fmaf(part[0][0] + part[1][0], ts0 * sa, acc[0]);
+  acc[1] = fmaf(part[0][1] + part[1][1], ts1 * sa, acc[1]);
+  acc[2] = fmaf(part[0][2] + part[1][2], ts0 * sb, acc[2]);
+  acc[3] = fmaf(part[0][3] + part[1][3], ts1 * sb, acc[3]);
 }
 
 template <class Cfg>
@@ -545,18 +556,27 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         float to, back;
         moe_act_scale(m, to, back);
         if (task < tasks) {
+          uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + col * 64;
+          auto put = [&](uint8_t* row, const uint32_t (&w)[4]) {
+            if constexpr (MX) {
+              // a lane's codes are 8 consecutive values
+              *reinterpret_cast<uint4*>(row + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+              // a lane's codes are 4 consecutive values of each 16
+              uint8_t* at = row + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
+              *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
+              *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
+            }
+          };
           uint32_t w[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[i] = pack_f16x2(v[u][2 * i] * to, v[u][2 * i + 1] * to);
-          uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + col * 64;
-          if constexpr (MX) {
-            // a lane's codes are 8 consecutive values
-            *reinterpret_cast<uint4*>(to16 + (l16 & 3) * 16) = make_uint4(w[0], w[1], w[2], w[3]);
-          } else {
-            // a lane's codes are 4 consecutive values of each 16
-            uint8_t* at = to16 + ((l16 >> 1) & 1) * 8 + (l16 & 1) * 32;
-            *reinterpret_cast<uint2*>(at) = make_uint2(w[0], w[1]);
-            *reinterpret_cast<uint2*>(at + 16) = make_uint2(w[2], w[3]);
+          put(to16, w);
+          if constexpr (!GATE) {  // (beside an infinity or a NaN nothing else counts)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = m < 0x7F800000u ? f16x2_rest(v[u][2 * i] * to, v[u][2 * i + 1] * to, w[i]) : 0u;
+            put(to16 + p.low, w);
           }
           if (l16 == 0) ts[b * kMoeChunk + col] = back;
         }
@@ -679,16 +699,18 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
     uint32_t phase = 0u;
     bool ok = true;
     // Block FP8 scales: lane l holds those of K blocks l and l + 32 of the
-    // unit's two 8-row halves, requested a unit ahead where they change.
-    float sc[2][2] = {}, sc_next[2][2] = {};
+    // unit's two 8-row halves, requested a unit ahead where they change.  (DOWN:
+    // both halves have the same, and a K range at most 32 blocks.)
+    constexpr int SC = GATE ? 2 : 1;
+    float sc[SC][SC] = {}, sc_next[SC][SC] = {};
     auto load_scales = [&](int chunk, int seg, int tile) {
       const float* e = static_cast<const float*>(p.ws) + int64_t(route.chunk_expert[chunk]) * p.rb * p.kb;
       const int kb = seg * (p.seg_len / 128);
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int r = GATE ? half * p.I + tile * 8 : tile * 16 + 8 * half;
+      for (int half = 0; half < SC; ++half) {
+        const int r = GATE ? half * p.I + tile * 8 : tile * 16;
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < SC; ++j) {
           const int b = kb + lane + 32 * j;
           sc_next[half][j] = b < p.kb ? ldg_pinned(e + int64_t(r >> 7) * p.kb + b) : 0.f;
         }
@@ -696,15 +718,33 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
     };
     Walk w = begin();
     if (!MX && w.u < u1 && group < w.count) load_scales(w.chunk, w.seg, w.tile + group);
-    if constexpr (!GATE) griddep_wait();  // h
+    // Where this lane's fragments and its two columns' scales are.
+    uint32_t b_cols = b_lane;
+    int col0 = 2 * t4, col1 = 2 * t4 + 1, columns_of = -1;
+    bool beside = false;
     for (; w.u < u1; next(w)) {
       const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
       const int k_len = min(p.seg_len, K - seg * p.seg_len);
       const int blocks = (k_len + 127) / 128;
       const int key = p.resident ? seg : chunk * p.segments + seg;
+      if (!GATE && columns_of != chunk) {
+        columns_of = chunk;
+        const int pairs = route.chunk_count[chunk], list = route.chunk_first[chunk];
+        beside = pairs <= kMoeBeside;
+        auto column = [&](int j) {  // of the chunk's pair j
+          return beside && p.resident ? int(route.list[list + j]) : j;
+        };
+        // (a column without a pair reads some pair's)
+        b_cols = base + p.off_b + uint32_t(t4 * 16) +
+                 (beside ? uint32_t(column(min(g & 3, pairs - 1)) * 64) + (g >= kMoeBeside ? p.low : 0u)
+                         : uint32_t(min(g, p.cols - 1) * 64));
+        col0 = column(beside ? min(2 * t4 & 3, pairs - 1) : 2 * t4);
+        col1 = column(beside ? min((2 * t4 + 1) & 3, pairs - 1) : 2 * t4 + 1);
+      }
       if (have != key) {
         count = p.resident ? p.cols : route.chunk_count[chunk];
         if (!GATE || !p.resident) {
+          if constexpr (!GATE) griddep_wait();  // h
           named_bar_sync(1, 32 * W);  // every warp is done with the last ones
           fragments(count, k_len, [&](int col) {
             const int pair = p.resident ? col : route.list[route.chunk_first[chunk] + col];
@@ -717,7 +757,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
       }
       if constexpr (!MX) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) sc[half][0] = sc_next[half][0], sc[half][1] = sc_next[half][1];
+        for (int half = 0; half < SC; ++half)
+#pragma unroll
+          for (int j = 0; j < SC; ++j) sc[half][j] = sc_next[half][j];
         // the next row's unit of this group (if it has none, what is loaded is not used)
         Walk v = w;
         next(v);
@@ -741,6 +783,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         // One 128-wide K block: its scales of rows g and g + 8, this lane's
         // ldmatrix row (lanes 0-7 / 8-15 the two halves' rows in one 16-byte
         // chunk, lanes 16-31 in the next), its token fragments and scales.
+        uint32_t part = b_cols;
         auto block = [&](int i, auto full_tag, int steps) {
           constexpr bool FULL = decltype(full_tag)::value;
           const int b = b0 + i;
@@ -750,25 +793,35 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
             e8m0x4_to_float(ld_shared_u32(word + word_a), fa);
             e8m0x4_to_float(ld_shared_u32(word + word_b), fb);
           } else {
-            fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][1], b & 31);
-            fb[0] = GATE ? __shfl_sync(~0u, b < 32 ? sc[1][0] : sc[1][1], b & 31) : fa[0];
+            fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][SC - 1], b & 31);
+            fb[0] = GATE ? __shfl_sync(~0u, b < 32 ? sc[SC - 1][0] : sc[SC - 1][SC - 1], b & 31) : fa[0];
           }
           const uint32_t a_row = stage + a_lane + uint32_t(MX ? i >> 1 : i) * 1024u;
           const uint32_t chunk0 = (MX ? (i & 1) * 4u : 0u) + (lane >> 4);
-          moe_block<Cfg, FULL>(acc, a_row, chunk0, b_lane + uint32_t(b * 4) * piece, piece, steps, fa, fb,
-                               ts + b * kMoeChunk + 2 * t4);
+          float ts0, ts1;
+          if constexpr (GATE) {
+            const float2 t = *reinterpret_cast<const float2*>(ts + b * kMoeChunk + 2 * t4);
+            ts0 = t.x, ts1 = t.y;
+          } else {
+            ts0 = ts[b * kMoeChunk + col0], ts1 = ts[b * kMoeChunk + col1];
+          }
+          moe_block<Cfg, FULL>(acc, a_row, chunk0, part + uint32_t(b * 4) * piece, piece, steps, fa, fb, ts0, ts1);
         };
         // Whole blocks two at a time (their loads and MMA chains overlap),
         // then what is left; the last block of K may be short.
         const int whole = min(nb, (k_len - b0 * 128) / 128);
-        int i = warp_in_group;
-        for (; i + kStep < whole; i += 2 * kStep) {
-          block(i, std::true_type(), 4);
-          block(i + kStep, std::true_type(), 4);
-        }
-        for (; i < nb; i += kStep) {
-          if (i < whole) block(i, std::true_type(), 4);
-          else block(i, std::false_type(), (k_len - (b0 + i) * 128) / 32);
+        while (true) {
+          int i = warp_in_group;
+          for (; i + kStep < whole; i += 2 * kStep) {
+            block(i, std::true_type(), 4);
+            block(i + kStep, std::true_type(), 4);
+          }
+          for (; i < nb; i += kStep) {
+            if (i < whole) block(i, std::true_type(), 4);
+            else block(i, std::false_type(), (k_len - (b0 + i) * 128) / 32);
+          }
+          if (GATE || beside || part != b_cols) break;
+          part += p.low;  // a second pass for the lower parts
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
@@ -821,7 +874,12 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
           }
         };
         // this lane has columns 2 t4 and the next
-        if (p.resident) {
+        const bool beside = !GATE && count <= kMoeBeside;
+        if (beside) {  // the lower parts are four columns further on
+          v.x += __shfl_down_sync(~0u, v.x, 2), v.y += __shfl_down_sync(~0u, v.y, 2);
+          v.z += __shfl_down_sync(~0u, v.z, 2), v.w += __shfl_down_sync(~0u, v.w, 2);
+        }
+        if (p.resident && !beside) {
           for (int k = 0; k < count; ++k) {
             const int col = GATE ? pairs[k] / p.top_k : pairs[k];
             if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);

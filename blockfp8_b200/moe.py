@@ -9,9 +9,12 @@
          MXFP4:      uint8 codes [E, rows, K / 2] with scale tiles
                      [E, ceil(rows / 128), ceil(K / 128), 32, 16]
 
-Activations are not quantized: at these sizes the weights are the traffic, and
-keeping x and h in 16 bits costs nothing.  (The dense block-FP8 linear
-quantizes its activations; a layer built from it differs by that rounding.)
+Activations are not quantized: at these sizes the weights are the traffic.  x
+enters the products as f16 with one power of two per token and 128 values,
+which holds bf16 exactly down to 2^-28 of the largest of them; h as two such
+parts, 22 bits of each value (2^-39 of the largest at worst).  (The dense
+block-FP8 linear quantizes its activations; a layer built from it differs by
+that rounding.)
 Two kernels and no synchronisation; results do not depend on the order in
 which CTAs finish.  H and I are multiples of 32, H at most 8192, E at most
 512, top_k at most 16.  The kernels check their arguments themselves
