@@ -481,6 +481,28 @@ __device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint3
   acc[3] = fmaf(part[0][3] + part[1][3], ts1 * sb, acc[3]);
 }
 
+// The producer that fills a slot: a ring belongs to one group, a group to one
+// producer.  It alone may drain the slot: to another one its passes are still
+// running, and a parity tells a pass only from its neighbours.
+__host__ __device__ constexpr int moe_producer_of(int slot, int ring, int producers) { return slot / ring % producers; }
+constexpr bool moe_producers_agree(int groups, int producers) {
+  for (int ring = 2; ring * groups <= 16; ++ring)
+    for (int slot = 0; slot < ring * groups; ++slot) {
+      int owners = 0;
+      for (int w = 0; w < producers; ++w)
+        for (int k = 0; k < groups / producers; ++k) {  // as the producers walk them
+          const int g = w + k * producers;
+          if (slot >= g * ring && slot < (g + 1) * ring) {
+            if (moe_producer_of(slot, ring, producers) != w) return false;
+            ++owners;
+          }
+        }
+      if (owners != 1) return false;
+    }
+  return true;
+}
+static_assert(moe_producers_agree(2, 1) && moe_producers_agree(4, 2), "a slot has one producer");
+
 template <class Cfg>
 __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(const __grid_constant__ MoeParams p) {
   constexpr bool GATE = Cfg::GATE, MX = Cfg::MX;
@@ -684,9 +706,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
       }
     }
     __syncwarp();
-    // Every copy issued lands before the CTA may exit (the consumers have
-    // waited for them all, unless a wait gave up).
-    if (lane < S && issued[lane] > 0) mbar_wait(full(lane), uint32_t(issued[lane] - 1) & 1u, nullptr, kMoeWaitDrain);
+    // Every copy this warp issued lands before the CTA may exit (the consumers
+    // have waited for them all, unless a wait gave up).
+    if (lane < S && moe_producer_of(lane, ring, PRODUCERS) == warp - W && issued[lane] > 0)
+      mbar_wait(full(lane), uint32_t(issued[lane] - 1) & 1u, nullptr, kMoeWaitDrain);
     __syncwarp();
   } else if (warp < W) {
     // ---------------------------------------------------------------- consumers
