@@ -155,7 +155,7 @@ int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaS
 
 constexpr int kMoeMaxHidden = 8192;
 constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
-constexpr int kMoeBusySegment = 2048;  // the same with eight columns: 64 KB, which leaves the ring its depth
+constexpr int kMoeBusySegment = 2048;  // the same in two planes: 64 KB, which leaves the ring its depth
 constexpr int kMoeHalfSmem = 113 * 1024;
 constexpr int kMoeSharedSmem = 226 * 1024;  // of two CTAs on an SM, without what the system takes
 
@@ -163,13 +163,13 @@ constexpr int kMoeSharedSmem = 226 * 1024;  // of two CTAs on an SM, without wha
 // are laid out.
 struct MoeLayout {
   int segments, seg_len, box, unit_stages, stages, smem, cols, resident;
-  uint32_t off_b, off_ts, off_red, off_route, off_bars, low;
+  uint32_t off_b, off_ts, off_red, off_route, off_bars, plane;
 };
 
 // K of `k` values in `segments` ranges, `entries` tokens or pairs that could
-// have a column of their own (in `parts` f16 parts), in stages of up to max_box
-// 128-byte columns and within `limit` bytes of shared memory.
-bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int parts, int warps, int max_box, int limit,
+// have a column of their own (DOWN: two), in stages of up to max_box 128-byte
+// columns and within `limit` bytes of shared memory.
+bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, bool down, int warps, int max_box, int limit,
                 MoeLayout* out) {
   const int P = p.T * p.top_k, per_column = p.format ? 256 : 128;  // values of a 128-byte column
   const int columns = cdiv(cdiv(k, per_column), segments), unit_stages = cdiv(columns, max_box);
@@ -177,11 +177,13 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
   out->unit_stages = unit_stages;
   out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
   out->segments = cdiv(k, out->seg_len);
-  out->resident = entries <= kMoeChunk;
-  out->cols = out->resident ? entries : std::min(P, kMoeChunk);
+  out->resident = entries <= kMoeChunk && (!down || warps == 8);
+  out->cols = down ? (out->resident ? 2 * std::min(entries, kMoeBeside) : kMoeChunk)
+                   : out->resident ? entries : std::min(P, kMoeChunk);
+  const int planes = !down ? 1 : out->resident ? cdiv(entries, kMoeBeside) : warps == 8 ? 1 : 2;
   const int blocks = cdiv(std::min(k, out->seg_len), 128);
   const int stage = round_up(out->box * (2048 + (p.format ? 512 : 0)), 1024);
-  const int b = blocks * 256 * out->cols * parts, ts = blocks * kMoeChunk * 4;
+  const int b = blocks * 256 * out->cols * planes, ts = blocks * kMoeChunk * 4;
   const int red = kMoeRedBufs * warps * 512, route = round_up(moe_route_bytes(P), 16);
   const int scratch = P > 32 ? p.E * (cdiv(P, 32) + 1) * 4 : 0;
   auto end_of = [&](int stages) { return 8 * (2 * stages + 2 * warps / kMoeGroupWarps * kMoeRedBufs) + 16 + 4 * stages; };
@@ -194,7 +196,7 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, int
   if (fixed + ring > limit) return false;
   out->stages = stages;
   out->off_b = uint32_t(ring);
-  out->low = uint32_t(b / parts);
+  out->plane = uint32_t(b / planes);
   out->off_ts = out->off_b + uint32_t(b);
   out->off_red = out->off_ts + uint32_t(ts);
   out->off_route = out->off_red + uint32_t(red);
@@ -209,20 +211,21 @@ struct MoeShape {
 };
 
 bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
-  const int P = p.T * p.top_k, segments = cdiv(p.I, P > kMoeChunk / 2 ? kMoeBusySegment : kMoeSegment);
-  auto one = [&](int k, int ranges, int entries, int parts, int warps, int limit, MoeLayout* lay) {
+  const int P = p.T * p.top_k, busy = cdiv(p.I, kMoeBusySegment);
+  const int few = P > kMoeBeside && P <= kMoeChunk ? busy : cdiv(p.I, kMoeSegment);
+  auto one = [&](int k, int ranges, int entries, bool down, int warps, int limit, MoeLayout* lay) {
     s->warps = warps;
     for (int box = 8; box >= 1; box /= 2)
-      if (moe_layout(p, k, ranges, entries, parts, warps, box, limit, lay)) return true;
+      if (moe_layout(p, k, ranges, entries, down, warps, box, limit, lay)) return true;
     return false;
   };
   // Up to 8 tokens: GATE in half an SM's shared memory and DOWN in what it
   // leaves, so that DOWN starts beside GATE and requests its weights while GATE
   // runs.
-  if (p.T <= 8 && one(p.H, 1, p.T, 1, 8, kMoeHalfSmem, &s->gate) &&
-      one(p.I, segments, P, 2, 8, kMoeSharedSmem - s->gate.smem, &s->down))
+  if (p.T <= 8 && one(p.H, 1, p.T, false, 8, kMoeHalfSmem, &s->gate) &&
+      one(p.I, few, P, true, 8, kMoeSharedSmem - s->gate.smem, &s->down))
     return true;
-  return one(p.H, 1, p.T, 1, 16, kMaxSmem, &s->gate) && one(p.I, segments, P, 2, 16, kMaxSmem, &s->down);
+  return one(p.H, 1, p.T, false, 16, kMaxSmem, &s->gate) && one(p.I, busy, P, true, 16, kMaxSmem, &s->down);
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
@@ -315,7 +318,7 @@ int launch_moe_kernel(MoeParams& mp, const MoeLayout& lay, int dev, int num_sms,
   mp.off_red = lay.off_red;
   mp.off_route = lay.off_route;
   mp.off_bars = lay.off_bars;
-  mp.low = lay.low;
+  mp.plane = lay.plane;
   mp.cols = lay.cols;
   mp.resident = lay.resident;
   cudaLaunchConfig_t cfg{};

@@ -45,9 +45,10 @@
 //   at 2^14: bf16 values are exact down to 2^-28 of it.  h (fp32) takes two
 //   f16 parts, the value rounded and what that leaves: 22 bits of each value,
 //   at worst 2^-39 of the largest.  Up to four pairs have their upper parts in
-//   the MMA's columns 0-3 and the lower ones in 4-7; more take a second pass over
-//   the stage.  (Both parts against the weights once converted: spills, and 1 us
-//   of 28 for one token, which needs no second pass.)
+//   the MMA's columns 0-3 and the lower ones in 4-7.  Batches beyond 8 tokens have
+//   chunks of up to eight, whose parts lie in two planes of eight columns and
+//   take MMAs of their own (and a unit of them about an eighth more time: the
+//   CTAs' shares of units count them as such).
 // - A last warp finishes units: it adds the consumers' sums in warp order.
 //   z goes to memory and a small third kernel adds each token's pairs in j
 //   order.  (Counting arrivals and letting the last unit of an output row tile
@@ -72,6 +73,7 @@ namespace bfp8 {
 constexpr int kMoeMaxTokens = 64;
 constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeMaxExperts = 512;
+constexpr int kMoeBeside = 4;  // most pairs whose h has both parts in one MMA's columns
 
 struct MoeParams {
   const void* x;  // [T, H] bf16 or fp16
@@ -102,7 +104,7 @@ struct MoeParams {
   int cols;               // token columns held
   int resident;           // every token (GATE) or pair (DOWN) has its own
   uint32_t off_b, off_ts, off_red, off_route, off_bars;  // shared memory
-  uint32_t low;  // DOWN: from h's upper parts to its lower ones
+  uint32_t plane;  // DOWN: bytes of a plane of columns
 };
 
 struct MoeSumParams {
@@ -230,10 +232,11 @@ __device__ __forceinline__ void moe_select(const MoeParams& p, const MoeRoute& r
   }
 }
 
-// The chunk tables, by all threads of the CTA; at most cap pairs a chunk.
+// The chunk tables, by all threads of the CTA; at most cap pairs a chunk, and
+// (P <= 8) all of one half of the pairs where `halves` says so.
 // scratch: room for E (ceil(P / 32) + 1) words.
 template <int THREADS>
-__device__ __forceinline__ void moe_group(const MoeParams& p, const MoeRoute& r, uint32_t* scratch, int cap) {
+__device__ __forceinline__ void moe_group(const MoeParams& p, const MoeRoute& r, uint32_t* scratch, int cap, bool halves) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int P = p.T * p.top_k, words = (P + 31) / 32;
   uint32_t* masks = scratch;                                     // [E][words] pairs of each expert
@@ -245,7 +248,7 @@ __device__ __forceinline__ void moe_group(const MoeParams& p, const MoeRoute& r,
     // One warp, a pair a lane; an expert's chunks stand where its first pair does.
     if (warp == 0) {
       const int e = lane < P ? r.expert[lane] : -1;
-      const uint32_t same = __match_any_sync(~0u, e);
+      const uint32_t same = __match_any_sync(~0u, halves && e >= 0 ? 2 * e + lane / kMoeBeside : e);
       const int n = e >= 0 ? __popc(same) : 0, at = __popc(same & ((1u << lane) - 1u));
       const bool first = n > 0 && at == 0;
       int pairs = first ? n : 0, chunks = first ? (n + cap - 1) / cap : 0;
@@ -405,7 +408,6 @@ __global__ void __launch_bounds__(kMoeSumThreads) moe_sum_kernel(const MoeSumPar
 }
 
 constexpr int kMoeChunk = 8;       // most pairs of a chunk: the MMA's columns
-constexpr int kMoeBeside = 4;      // most pairs whose h has both parts in one MMA's columns
 constexpr int kMoeGroupWarps = 4;  // consumer warps of a group, which works on a unit of its own
 constexpr int kMoeRedBufs = 2;     // buffers of the warps' sums (512 bytes a warp)
 
@@ -417,6 +419,9 @@ struct MoeCfg {
   static constexpr int PRODUCERS = WARPS == 16 ? 2 : 1;
   static constexpr int THREADS = 32 * (WARPS + PRODUCERS + 1);
   static constexpr int CTAS_PER_SM = WARPS == 8 ? 2 : 1;
+  // DOWN's chunks may have more than four pairs; otherwise all pairs may have
+  // columns of their own.
+  static constexpr bool BUSY = !GATE && WARPS == 16;
   using T = T_;                   // x and y
   static constexpr int BLOCK_BYTES = MX ? 64 : 128;  // 128 values of K of one row
 };
@@ -424,12 +429,12 @@ struct MoeCfg {
 // acc += one 128-wide K block of 16 weight rows times the chunk's 8 columns.
 // a_row, chunk0: this lane's ldmatrix row and first 16-byte chunk in it;
 // b_addr: its piece of the tokens' fragments, piece bytes apart per 32 values
-// of K; ts0, ts1: the scales of this lane's two columns.  FULL: all four 32-wide steps, so that every load can go out first;
-// else `steps` of them.
-template <class Cfg, bool FULL>
+// of K; LOW: as much again `low` further on, for the same columns; ts: the scales of this lane's two columns.  FULL: all four 32-wide steps, so
+// that every load can go out first; else `steps` of them.
+template <class Cfg, bool FULL, bool LOW>
 __device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint32_t chunk0, uint32_t b_addr,
-                                          uint32_t piece, int steps, const float (&fa)[4],
-                                          const float (&fb)[4], float ts0, float ts1) {
+                                          uint32_t piece, uint32_t low, int steps, const float (&fa)[4],
+                                          const float (&fb)[4], const float* ts) {
   // the 128-byte swizzle: chunk XOR row inside 8 rows
   auto chunk_at = [&](uint32_t c) { return a_row + (((chunk0 + c) ^ (threadIdx.x & 7u)) << 4); };
   float part[2][4] = {};
@@ -452,6 +457,11 @@ __device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint3
         float d[4] = {0.f, 0.f, 0.f, 0.f};
         mma_f16(d, ha[0], hb[0], ha[1], hb[1], b.x, b.y);
         mma_f16(d, ha[2], hb[2], ha[3], hb[3], b.z, b.w);
+        if constexpr (LOW) {
+          const uint4 l = ld_shared_v4(b_addr + low + uint32_t(s) * piece);
+          mma_f16(d, ha[0], hb[0], ha[1], hb[1], l.x, l.y);
+          mma_f16(d, ha[2], hb[2], ha[3], hb[3], l.z, l.w);
+        }
         float(&q)[4] = part[s & 1];
         q[0] = fmaf(d[0], fa[s], q[0]);
         q[1] = fmaf(d[1], fa[s], q[1]);
@@ -472,13 +482,47 @@ __device__ __forceinline__ void moe_block(float (&acc)[4], uint32_t a_row, uint3
         const uint4 b = ld_shared_v4(b_addr + uint32_t(s) * piece);
         mma_f16(part[0], lo[0], lo[1], hi[0], hi[1], b.x, b.y);
         mma_f16(part[1], lo[2], lo[3], hi[2], hi[3], b.z, b.w);
+        if constexpr (LOW) {
+          const uint4 l = ld_shared_v4(b_addr + low + uint32_t(s) * piece);
+          mma_f16(part[0], lo[0], lo[1], hi[0], hi[1], l.x, l.y);
+          mma_f16(part[1], lo[2], lo[3], hi[2], hi[3], l.z, l.w);
+        }
       }
   }
   const float sa = Cfg::MX ? 1.f : fa[0], sb = Cfg::MX ? 1.f : fb[0];
-  acc[0] = fmaf(part[0][0] + part[1][0], ts0 * sa, acc[0]);
-  acc[1] = fmaf(part[0][1] + part[1][1], ts1 * sa, acc[1]);
-  acc[2] = fmaf(part[0][2] + part[1][2], ts0 * sb, acc[2]);
-  acc[3] = fmaf(part[0][3] + part[1][3], ts1 * sb, acc[3]);
+  const float2 t = *reinterpret_cast<const float2*>(ts);
+  acc[0] = fmaf(part[0][0] + part[1][0], t.x * sa, acc[0]);
+  acc[1] = fmaf(part[0][1] + part[1][1], t.y * sa, acc[1]);
+  acc[2] = fmaf(part[0][2] + part[1][2], t.x * sb, acc[2]);
+  acc[3] = fmaf(part[0][3] + part[1][3], t.y * sb, acc[3]);
+}
+
+// A stage as a consumer warp sees it, and one of its 128-wide K blocks: the
+// block's scales of rows g and g + 8, this lane's ldmatrix row (lanes 0-7 / 8-15
+// the two halves' rows in one 16-byte chunk, lanes 16-31 in the next), its
+// token fragments and scales.
+struct MoeStage {
+  uint32_t base, words, word_a, word_b;  // MXFP4: of the scales, and in them the halves' words
+  uint32_t a_lane, b_cols, piece, low;
+  const float* ts;
+  int b0;  // its first block's place in the K range
+};
+template <class Cfg, bool FULL, bool LOW, int SC>
+__device__ __forceinline__ void moe_stage_block(const MoeStage& st, int i, int steps, const float (&sc)[SC][SC], float (&acc)[4]) {
+  const int lane = threadIdx.x & 31, b = st.b0 + i;
+  float fa[4], fb[4];
+  if constexpr (Cfg::MX) {
+    const uint32_t word = st.base + st.words + uint32_t(i * 128 + (lane >> 2) * 16);
+    e8m0x4_to_float(ld_shared_u32(word + st.word_a), fa);
+    e8m0x4_to_float(ld_shared_u32(word + st.word_b), fb);
+  } else {
+    fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][SC - 1], b & 31);
+    fb[0] = Cfg::GATE ? __shfl_sync(~0u, b < 32 ? sc[SC - 1][0] : sc[SC - 1][SC - 1], b & 31) : fa[0];
+  }
+  const uint32_t a_row = st.base + st.a_lane + uint32_t(Cfg::MX ? i >> 1 : i) * 1024u;
+  const uint32_t chunk0 = (Cfg::MX ? (i & 1) * 4u : 0u) + (lane >> 4);
+  moe_block<Cfg, FULL, LOW>(acc, a_row, chunk0, st.b_cols + uint32_t(b * 4) * st.piece, st.piece, st.low, steps, fa, fb,
+                            st.ts + b * kMoeChunk);
 }
 
 // The producer that fills a slot: a ring belongs to one group, a group to one
@@ -514,6 +558,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   uint8_t* smem = smem_raw + (base - raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int S = p.stages;
+  const bool resident = !Cfg::BUSY && p.resident;
   // a stage: [half][column][8 rows][128 bytes], MXFP4: then [half][K block][8 rows][16 bytes] of scales
   const uint32_t half_bytes = uint32_t(p.box) * 1024u;
   const uint32_t scale_copy = MX ? uint32_t(p.box) * 256u : 0u;  // of a half
@@ -548,7 +593,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   // Activations in shared memory as f16 in MMA fragment order,
   // [32 values of K][token column][lane quarter][16 bytes], and one power of
   // two per column and 128-wide block.  A column past the batch reads some
-  // other token's values and is not used.
+  // other token's values and is not used.  DOWN: upper parts in the first half of
+  // a plane's columns and lower ones in the second, four pairs a plane; or, for a
+  // chunk of more, upper and lower ones in a plane each.
   uint8_t* bfrag = smem + p.off_b;
   float* ts = reinterpret_cast<float*>(smem + p.off_ts);  // [block][8]
   const uint32_t piece = uint32_t(p.cols) * 64u;
@@ -578,7 +625,10 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         float to, back;
         moe_act_scale(m, to, back);
         if (task < tasks) {
-          uint8_t* to16 = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece + col * 64;
+          uint8_t* block = bfrag + uint32_t(b * 4 + (l16 >> 2)) * piece;
+          const bool planes = Cfg::BUSY && columns > kMoeBeside;
+          const int at = GATE || planes ? col : col % kMoeBeside;
+          uint8_t* to16 = block + at * 64 + (GATE || planes ? 0u : col / kMoeBeside * p.plane);
           auto put = [&](uint8_t* row, const uint32_t (&w)[4]) {
             if constexpr (MX) {
               // a lane's codes are 8 consecutive values
@@ -598,7 +648,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               w[i] = m < 0x7F800000u ? f16x2_rest(v[u][2 * i] * to, v[u][2 * i + 1] * to, w[i]) : 0u;
-            put(to16 + p.low, w);
+            put(to16 + (planes ? p.plane : piece / 2), w);
           }
           if (l16 == 0) ts[b * kMoeChunk + col] = back;
         }
@@ -610,10 +660,11 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   // out once, and a chunk uses its pairs' columns; else a chunk's pairs are laid
   // out when a unit of it comes up.
   moe_select<THREADS>(p, route);
-  if (GATE && p.resident && warp < W)
+  if (GATE && resident && warp < W)
     fragments(p.T, p.H, [&](int t) { return static_cast<const T*>(p.x) + int64_t(t) * p.ldx; });
   // (scratch: the ring, before its first copy)
-  moe_group<THREADS>(p, route, reinterpret_cast<uint32_t*>(smem), p.resident ? p.T * p.top_k : p.cols);
+  moe_group<THREADS>(p, route, reinterpret_cast<uint32_t*>(smem),
+                     resident ? p.T * p.top_k : GATE || Cfg::BUSY ? p.cols : kMoeBeside, !GATE && resident);
 
   if (GATE && blockIdx.x == 0)
     for (int i = tid; i < p.T * p.top_k; i += THREADS)
@@ -621,8 +672,30 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   const int chunks = route.totals[0];
   const int tiles = GATE ? p.I / 8 : p.H / 16, per_chunk = tiles * p.segments;
   const int K = GATE ? p.H : p.I;
-  const int64_t units = int64_t(chunks) * per_chunk;
-  const int u0 = int(units * blockIdx.x / gridDim.x), u1 = int(units * (blockIdx.x + 1) / gridDim.x);
+  // CTA b of G has units [x b / G, x (b + 1) / G) of all x = chunks * per_chunk;
+  // with BUSY, places where a unit of five pairs or more counts 9 and others 8.
+  auto first_unit = [&](int b) {
+    if constexpr (!Cfg::BUSY) {
+      return int(int64_t(chunks) * per_chunk * b / gridDim.x);
+    } else {
+      auto busy_of = [&](int c) { return __ballot_sync(~0u, c < chunks && route.chunk_count[c] > kMoeBeside); };
+      int total = 8 * chunks;
+      for (int c = 0; c < chunks; c += 32) total += __popc(busy_of(c + lane));
+      const int64_t place = int64_t(total) * per_chunk * b / gridDim.x;
+      int64_t before = 0;
+      for (int c = 0; c < chunks; c += 32) {
+        const uint32_t busy = busy_of(c + lane);
+        const int n = min(32, chunks - c), own = busy >> lane & 1u ? 9 : 8;
+        const int64_t at = before + int64_t(8 * lane + __popc(busy & ((1u << lane) - 1u))) * per_chunk;
+        const uint32_t mine = __ballot_sync(~0u, lane < n && place >= at && place < at + int64_t(own) * per_chunk);
+        const int u = (c + lane) * per_chunk + int((place - at) / own);
+        if (mine) return __shfl_sync(~0u, u, __ffs(mine) - 1);
+        before += int64_t(8 * n + __popc(busy)) * per_chunk;
+      }
+      return chunks * per_chunk;
+    }
+  };
+  const int u0 = first_unit(blockIdx.x), u1 = first_unit(blockIdx.x + 1);
   // The walk over this CTA's units, a row of up to G of them (one a group) with
   // the same chunk and K range at a time.
   struct Walk {
@@ -714,7 +787,8 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   } else if (warp < W) {
     // ---------------------------------------------------------------- consumers
     const int g = lane >> 2, t4 = lane & 3;
-    const uint32_t b_lane = base + p.off_b + uint32_t(min(g, p.cols - 1) * 64 + t4 * 16);
+    auto column = [&](int n) { return min(g % kMoeBeside, n - 1) + (g < kMoeBeside ? 0 : n); };  // n and n, upper and lower
+    const uint32_t b_lane = base + p.off_b + uint32_t((GATE ? min(g, p.cols - 1) : column(p.cols / 2)) * 64 + t4 * 16);
     constexpr int kStep = kMoeGroupWarps;
     const int group = warp / kStep, warp_in_group = warp % kStep;
     const uint32_t a_lane = ((lane >> 3) & 1) * half_bytes + (lane & 7) * 128u;
@@ -739,38 +813,26 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         }
       }
     };
+    MoeStage st;
+    st.words = 2u * half_bytes;
+    st.a_lane = a_lane, st.piece = piece, st.low = p.plane;
+    st.b_cols = b_lane, st.ts = ts + 2 * t4;
+    bool busy = false;
+    int columns_of = -1;
     Walk w = begin();
     if (!MX && w.u < u1 && group < w.count) load_scales(w.chunk, w.seg, w.tile + group);
-    // Where this lane's fragments and its two columns' scales are.
-    uint32_t b_cols = b_lane;
-    int col0 = 2 * t4, col1 = 2 * t4 + 1, columns_of = -1;
-    bool beside = false;
     for (; w.u < u1; next(w)) {
       const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
       const int k_len = min(p.seg_len, K - seg * p.seg_len);
       const int blocks = (k_len + 127) / 128;
-      const int key = p.resident ? seg : chunk * p.segments + seg;
-      if (!GATE && columns_of != chunk) {
-        columns_of = chunk;
-        const int pairs = route.chunk_count[chunk], list = route.chunk_first[chunk];
-        beside = pairs <= kMoeBeside;
-        auto column = [&](int j) {  // of the chunk's pair j
-          return beside && p.resident ? int(route.list[list + j]) : j;
-        };
-        // (a column without a pair reads some pair's)
-        b_cols = base + p.off_b + uint32_t(t4 * 16) +
-                 (beside ? uint32_t(column(min(g & 3, pairs - 1)) * 64) + (g >= kMoeBeside ? p.low : 0u)
-                         : uint32_t(min(g, p.cols - 1) * 64));
-        col0 = column(beside ? min(2 * t4 & 3, pairs - 1) : 2 * t4);
-        col1 = column(beside ? min((2 * t4 + 1) & 3, pairs - 1) : 2 * t4 + 1);
-      }
+      const int key = resident ? seg : chunk * p.segments + seg;
       if (have != key) {
-        count = p.resident ? p.cols : route.chunk_count[chunk];
-        if (!GATE || !p.resident) {
+        count = resident ? p.T * p.top_k : route.chunk_count[chunk];
+        if (!GATE || !resident) {
           if constexpr (!GATE) griddep_wait();  // h
           named_bar_sync(1, 32 * W);  // every warp is done with the last ones
           fragments(count, k_len, [&](int col) {
-            const int pair = p.resident ? col : route.list[route.chunk_first[chunk] + col];
+            const int pair = resident ? col : route.list[route.chunk_first[chunk] + col];
             if constexpr (GATE) return static_cast<const T*>(p.x) + int64_t(pair / p.top_k) * p.ldx;
             else return p.h + int64_t(pair) * p.I + seg * p.seg_len;
           });
@@ -794,57 +856,45 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         }
       }
       if (group >= w.count) continue;
+      if (!GATE && columns_of != chunk) {  // which four pairs' plane, and the scales of columns 2 t4 mod 4
+        columns_of = chunk;
+        busy = Cfg::BUSY && count > kMoeBeside;
+        const int set = resident ? route.list[route.chunk_first[chunk]] / kMoeBeside : 0;
+        st.b_cols = b_lane + set * p.plane;
+        st.ts = ts + (busy ? 2 * t4 : 2 * (t4 & 1) + kMoeBeside * set);
+      }
       // MXFP4: the 32-row quarter of the rows' scale tiles
       const uint32_t word_a = uint32_t(((GATE ? tile * 8 : tile * 16) >> 5) & 3) * 4u;
       const uint32_t word_b = scale_copy + uint32_t(((GATE ? p.I + tile * 8 : tile * 16 + 8) >> 5) & 3) * 4u;
+      st.word_a = word_a, st.word_b = word_b;
       float acc[4] = {0.f, 0.f, 0.f, 0.f};
       for (int b0 = 0; b0 < unit_stages * stage_blocks; b0 += stage_blocks) {
         const int s = group * ring + slot;
         ok = mbar_wait(full(s), phase, abort_flag, kMoeWaitFull) && ok;
         const int nb = min(stage_blocks, blocks - b0);
-        const uint32_t stage = base + uint32_t(s) * stage_bytes;
-        // One 128-wide K block: its scales of rows g and g + 8, this lane's
-        // ldmatrix row (lanes 0-7 / 8-15 the two halves' rows in one 16-byte
-        // chunk, lanes 16-31 in the next), its token fragments and scales.
-        uint32_t part = b_cols;
-        auto block = [&](int i, auto full_tag, int steps) {
-          constexpr bool FULL = decltype(full_tag)::value;
-          const int b = b0 + i;
-          float fa[4], fb[4];
-          if constexpr (MX) {
-            const uint32_t word = stage + 2u * half_bytes + uint32_t(i * 128 + g * 16);
-            e8m0x4_to_float(ld_shared_u32(word + word_a), fa);
-            e8m0x4_to_float(ld_shared_u32(word + word_b), fb);
-          } else {
-            fa[0] = __shfl_sync(~0u, b < 32 ? sc[0][0] : sc[0][SC - 1], b & 31);
-            fb[0] = GATE ? __shfl_sync(~0u, b < 32 ? sc[SC - 1][0] : sc[SC - 1][SC - 1], b & 31) : fa[0];
+        st.base = base + uint32_t(s) * stage_bytes;
+        st.b0 = b0;
+        // Blocks are dealt over the whole unit, so that no warp has two more than
+        // another.
+        int i = (warp_in_group - b0) & (kStep - 1);
+        if (Cfg::BUSY && busy) {
+          for (; i < nb; i += kStep) {
+            const int steps = (k_len - (b0 + i) * 128) / 32;
+            if (steps >= 4) moe_stage_block<Cfg, true, Cfg::BUSY>(st, i, 4, sc, acc);
+            else moe_stage_block<Cfg, false, Cfg::BUSY>(st, i, steps, sc, acc);
           }
-          const uint32_t a_row = stage + a_lane + uint32_t(MX ? i >> 1 : i) * 1024u;
-          const uint32_t chunk0 = (MX ? (i & 1) * 4u : 0u) + (lane >> 4);
-          float ts0, ts1;
-          if constexpr (GATE) {
-            const float2 t = *reinterpret_cast<const float2*>(ts + b * kMoeChunk + 2 * t4);
-            ts0 = t.x, ts1 = t.y;
-          } else {
-            ts0 = ts[b * kMoeChunk + col0], ts1 = ts[b * kMoeChunk + col1];
-          }
-          moe_block<Cfg, FULL>(acc, a_row, chunk0, part + uint32_t(b * 4) * piece, piece, steps, fa, fb, ts0, ts1);
-        };
-        // Whole blocks two at a time (their loads and MMA chains overlap),
-        // then what is left; the last block of K may be short.
-        const int whole = min(nb, (k_len - b0 * 128) / 128);
-        while (true) {
-          int i = warp_in_group;
+        } else {
+          // Whole blocks two at a time (their loads and MMA chains overlap),
+          // then what is left; the last block of K may be short.
+          const int whole = min(nb, (k_len - b0 * 128) / 128);
           for (; i + kStep < whole; i += 2 * kStep) {
-            block(i, std::true_type(), 4);
-            block(i + kStep, std::true_type(), 4);
+            moe_stage_block<Cfg, true, false>(st, i, 4, sc, acc);
+            moe_stage_block<Cfg, true, false>(st, i + kStep, 4, sc, acc);
           }
           for (; i < nb; i += kStep) {
-            if (i < whole) block(i, std::true_type(), 4);
-            else block(i, std::false_type(), (k_len - (b0 + i) * 128) / 32);
+            if (i < whole) moe_stage_block<Cfg, true, false>(st, i, 4, sc, acc);
+            else moe_stage_block<Cfg, false, false>(st, i, (k_len - (b0 + i) * 128) / 32, sc, acc);
           }
-          if (GATE || beside || part != b_cols) break;
-          part += p.low;  // a second pass for the lower parts
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
@@ -897,14 +947,13 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
           }
         };
         // this lane has columns 2 t4 and the next
-        const bool beside = !GATE && count <= kMoeBeside;
-        if (beside) {  // the lower parts are four columns further on
+        if (!GATE && (!Cfg::BUSY || count <= kMoeBeside)) {  // the lower parts are four columns further on
           v.x += __shfl_down_sync(~0u, v.x, 2), v.y += __shfl_down_sync(~0u, v.y, 2);
           v.z += __shfl_down_sync(~0u, v.z, 2), v.w += __shfl_down_sync(~0u, v.w, 2);
         }
-        if (p.resident && !beside) {
+        if (resident) {
           for (int k = 0; k < count; ++k) {
-            const int col = GATE ? pairs[k] / p.top_k : pairs[k];
+            const int col = GATE ? pairs[k] / p.top_k : pairs[k] % kMoeBeside;
             if (col >> 1 == t4) store(pairs[k], col & 1 ? v.y : v.x, col & 1 ? v.w : v.z);
           }
         } else {
