@@ -198,19 +198,22 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
         mma_commit<1>(empty(s));
       }
       mma_commit<1>(done);
-      mbar_wait(done, 0, nullptr, kMxWaitDone);
+      if (!mbar_wait(done, 0, nullptr, kMxWaitDone)) *abort_flag = 1;
     }
     __syncwarp();
   } else {
     // Scales of stage i: its TMEM columns were last read by the MMAs whose end
     // let the producer refill the stage.
     const uint32_t t_lane = tmem + (uint32_t(32 * (warp & 3)) << 16) + uint32_t(Cfg::ACC_COLS);
+    bool ok = true;
     for (int i = 0; i < L; ++i) {
       const int s = i % S;
-      if (!mbar_wait(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull)) break;
+      // After a wait that gave up (the MMA thread's next one then does, too) a warp
+      // still meets the others at the barrier below.
+      if (ok) ok = mbar_wait_warp(full(s), uint32_t(i / S) & 1u, abort_flag, kMxWaitFull);
       if constexpr (QUANT) {
         // A thread takes 32 values of one token; tokens past M are zeros.
-        for (int task = threadIdx.x - 64; task < BN * 8; task += 128) {
+        for (int task = ok ? threadIdx.x - 64 : BN * 8; task < BN * 8; task += 128) {
           const int t = task >> 3, b = task & 7;
           uint32_t codes[4] = {0u, 0u, 0u, 0u}, byte = 0u;
           if (t < p.M) {
@@ -247,6 +250,7 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
         fence_proxy_async_smem();  // the MMAs read the codes through the async proxy
         named_bar_sync(1, 128);
       }
+      if (!ok) continue;
       uint32_t r[16];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -291,7 +295,10 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
   {
     griddep_wait();
     const int c0 = BN * rank / p.splits, c1 = BN * (rank + 1) / p.splits;
-    const bool ok = !*abort_flag;
+    // The sum is whole if no CTA of the cluster gave up.
+    bool ok = !*abort_flag;
+    if (p.splits > 1)
+      ok = !__any_sync(~0u, lane < p.splits && ld_cluster_u32(map_shared_rank(smem_u32(misc + 1), uint32_t(lane))) != 0u);
     for (int idx = threadIdx.x; idx < (c1 - c0) * 64; idx += Cfg::THREADS) {
       const int col = c0 + idx / 64, r2 = (idx & 63) * 2;
       const int m = mt * BN + col, n = nt * 128 + r2;
@@ -470,10 +477,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
       }
       // The leader's MMAs read what was loaded last; every copy has landed once
       // they are done.  (A CTA stays until its peer gets here, so that no
-      // commit arrives on a barrier that is gone.)
+      // commit arrives on a barrier that is gone.)  After a wait that gave up the
+      // leader waits for the copies themselves.
       for (int k = i > S ? i - S : 0; k < i; ++k) {
-        if (ok) mbar_wait(empty(k % S), uint32_t(k / S) & 1u, abort_flag, kMxWaitDrain);
-        else if (leader) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMxWaitDrain);  // a wait gave up
+        if (ok) ok = mbar_wait(empty(k % S), uint32_t(k / S) & 1u, abort_flag, kMxWaitDrain);
+        if (!ok && leader) mbar_wait(full(k % S), uint32_t(k / S) & 1u, nullptr, kMxWaitDrain);
       }
     }
     __syncwarp();
@@ -556,7 +564,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
           mma_commit_pair(empty(s));
           if (++s == S) s = 0, phase ^= 1u;
         }
-        mma_commit_pair(acc_full);
+        if (ok) mma_commit_pair(acc_full);  // a part of a sum is not stored, not by the peer either
       }
       mma_commit<2>(done);
       mbar_wait(done, 0, nullptr, kMxWaitDone);
@@ -570,8 +578,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
     const uint32_t out = base + uint32_t(Cfg::OFF_OUT + half * 128 * 64);
     const uint32_t empty_bar = leader_bars + 8u * uint32_t(4 * S + 1);
     int n = 0;
+    bool ok = true;
     for (int t = pair; t < tiles; t += pairs, ++n) {
-      if (!mbar_wait(acc_full, uint32_t(n) & 1u, abort_flag, kMxWaitAcc)) break;
+      // After a wait that gave up nothing is stored (the abort flag is up), but a
+      // warp still meets the others at the barriers below.
+      if (ok) ok = mbar_wait_warp(acc_full, uint32_t(n) & 1u, abort_flag, kMxWaitAcc);
       tc_fence_after();
       uint32_t packed[64];
 #pragma unroll
@@ -586,7 +597,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(MxPairCfg::THREADS, 
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(empty_bar);  // the next tile's MMAs may start
+      if (lane == 0 && ok) mbar_arrive_cluster(empty_bar);  // the next tile's MMAs may start
       int mt, nt;
       place(t, mt, nt);
 #pragma unroll

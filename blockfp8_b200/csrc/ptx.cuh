@@ -93,6 +93,11 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
   }
 }
 
+// The same by a whole warp, whose lanes agree: true if no lane gave up.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int* abort, uint32_t where) {
+  return __all_sync(~0u, mbar_wait(bar, parity, abort, where));
+}
+
 __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
@@ -556,7 +561,12 @@ __host__ __device__ constexpr uint32_t idesc_scale_half(int half) {
   return (uint32_t(2 * half) << 4) | (uint32_t(2 * half) << 29);
 }
 
-// The shared::cluster address's float (distributed shared memory).
+// The shared::cluster address's word, and floats (distributed shared memory).
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
