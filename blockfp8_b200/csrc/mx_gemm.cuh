@@ -251,6 +251,7 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
         named_bar_sync(1, 128);
       }
       if (!ok) continue;
+      tc_fence_after();  // those MMAs' reads come before the stores below
       uint32_t r[16];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {

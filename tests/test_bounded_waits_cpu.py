@@ -68,3 +68,25 @@ def test_waits_of_a_whole_warp_are_found(name):
     statements = _statements(os.path.join(CSRC, name))
     assert any("mbar_wait" in p and not _one_thread(h + [p]) for _, p, h, _ in statements)
     assert any("mbar_wait" in p and _one_thread(h + [p]) for _, p, h, _ in statements)
+
+
+TMEM_ACCESS = re.compile(r"\b(tmem_st16|tmem_ld16|tmem_ld32|mma_mxf4(<\w+>)?|tmem_cp_scales_pair)\(")
+
+
+def test_tensor_memory_is_touched_behind_a_fence():
+    """An mbarrier orders nothing in tensor memory by itself: between a wait and the next tcgen05 access of the
+    same thread stands tcgen05.fence::after_thread_sync."""
+    seen, bad = 0, []
+    waited = None
+    for line, piece, _, _ in _statements(os.path.join(CSRC, "mx_gemm.cuh")):
+        if "__global__" in piece:
+            waited = None
+        if "tc_fence_after()" in piece:
+            waited = None
+        if TMEM_ACCESS.search(piece):
+            seen += 1
+            if waited:
+                bad.append((line, f"wait in line {waited}", piece))
+        if re.search(r"\bmbar_wait(_warp)?\(", piece):
+            waited = line
+    assert seen >= 5 and not bad
