@@ -561,12 +561,7 @@ __host__ __device__ constexpr uint32_t idesc_scale_half(int half) {
   return (uint32_t(2 * half) << 4) | (uint32_t(2 * half) << 29);
 }
 
-// The shared::cluster address's word, and floats (distributed shared memory).
-__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
+// The shared::cluster address's float (distributed shared memory).
 __device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
