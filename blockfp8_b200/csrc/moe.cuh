@@ -925,7 +925,7 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         if (group >= w.count) break;
         const int chunk = w.chunk, seg = w.seg, tile = w.tile + group;
         const int buf = int(done[group] % RB);
-        if (!(ok = mbar_wait_warp(red_full(group, buf), done[group] / RB & 1u, abort_flag, kMoeWaitRedFull))) break;
+        ok = mbar_wait(red_full(group, buf), done[group] / RB & 1u, abort_flag, kMoeWaitRedFull);
         ++done[group];
         const int count = route.chunk_count[chunk];
         const short* pairs = route.list + route.chunk_first[chunk];
@@ -962,6 +962,9 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(red_empty(group, buf));
+        // (The lanes agree on a wait that gave up here, off the path to the stores:
+        // a vote behind the wait took 0.6 of 28 us for one token.)
+        if (!(ok = __all_sync(~0u, ok))) break;
       }
     }
   }
