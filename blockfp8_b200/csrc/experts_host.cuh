@@ -20,10 +20,14 @@ int element_size(int type) { return type == 0 ? 4 : 2; }
 
 int round_up(int x, int m) { return cdiv(x, m) * m; }
 
+// Sizes whose rounding up to tiles stays in 32 bits.
+constexpr int kMxMaxSize = INT32_MAX / 2;
+
 // ---- MXFP4 quantization -----------------------------------------------------------
 
 int check_codes(const void* q, int64_t ldq, const void* s, int M, int K) {
   if (M < 0 || K <= 0 || K % 32 != 0) return fail(BFP8_EINVAL, "K must be a positive multiple of 32");
+  if (M > kMxMaxSize || K > kMxMaxSize) return fail(BFP8_EINVAL, "too large");
   if (M == 0) return BFP8_OK;
   if (!q || !s) return fail(BFP8_EINVAL, "null operand pointer");
   if (!aligned16(q) || !aligned16(s) || ldq < K / 2 || ldq % 16 != 0)
@@ -154,6 +158,7 @@ int launch_mx_pair(const bfp8_mxfp4_gemm_problem& p, int dev, int num_sms, cudaS
 // ---- the expert layer ---------------------------------------------------------------
 
 constexpr int kMoeMaxHidden = 8192;
+constexpr int kMoeMaxInner = 1 << 24;
 constexpr int kMoeSegment = 4096;  // most K values whose activations DOWN keeps in shared memory
 constexpr int kMoeBusySegment = 2048;  // the same in two planes: 64 KB, which leaves the ring its depth
 constexpr int kMoeHalfSmem = 113 * 1024;
@@ -210,7 +215,7 @@ struct MoeShape {
   MoeLayout gate, down;
 };
 
-bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
+bool moe_layouts(const bfp8_moe_problem& p, MoeShape* s) {
   const int P = p.T * p.top_k, busy = cdiv(p.I, kMoeBusySegment);
   const int few = P > kMoeBeside && P <= kMoeChunk ? busy : cdiv(p.I, kMoeSegment);
   auto one = [&](int k, int ranges, int entries, bool down, int warps, int limit, MoeLayout* lay) {
@@ -226,6 +231,14 @@ bool moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
       one(p.I, few, P, true, 8, kMoeSharedSmem - s->gate.smem, &s->down))
     return true;
   return one(p.H, 1, p.T, false, 16, kMaxSmem, &s->gate) && one(p.I, busy, P, true, 16, kMaxSmem, &s->down);
+}
+
+int moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
+  if (!moe_layouts(p, s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
+  // every pair could be a chunk of its own
+  const int64_t units = int64_t(p.T) * p.top_k * std::max<int64_t>(p.I / 8, int64_t(p.H / 16) * s->down.segments);
+  if (units > INT32_MAX) return fail(BFP8_EINVAL, "too many units for one launch: fewer tokens or choices for an I this large");
+  return BFP8_OK;
 }
 
 // Tensor maps of one stack of expert weights [E, rows, k] and its scales.
@@ -281,7 +294,7 @@ int check_moe(const bfp8_moe_problem& p) {
   if (p.T < 1 || p.T > kMoeMaxTokens) return fail(BFP8_EINVAL, "the expert layer takes 1 to 64 tokens");
   if (p.H < 32 || p.H % 32 || p.H > kMoeMaxHidden)
     return fail(BFP8_EINVAL, "H must be a multiple of 32, at most 8192");
-  if (p.I < 32 || p.I % 32) return fail(BFP8_EINVAL, "I must be a positive multiple of 32");
+  if (p.I < 32 || p.I % 32 || p.I > kMoeMaxInner) return fail(BFP8_EINVAL, "I must be a positive multiple of 32, at most 2^24");
   if (p.E < 1 || p.E > kMoeMaxExperts) return fail(BFP8_EINVAL, "1 to 512 experts");
   if (p.top_k < 1 || p.top_k > kMoeMaxTopK || p.top_k > p.E)
     return fail(BFP8_EINVAL, "top_k must be at least 1 and at most min(16, E)");
@@ -399,6 +412,7 @@ int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* pp, void* stream) {
   if (quant) {
     if (p.M < 0 || p.M > BFP8_MXFP4_QUANT_MAX_M || p.K <= 0 || p.K % 32)
       return fail(BFP8_EINVAL, "16-bit activations: at most 16 rows, K a positive multiple of 32");
+    if (p.K > kMxMaxSize) return fail(BFP8_EINVAL, "too large");
     if (p.M && (!p.a || !aligned16(p.a) || p.lda < p.K || p.lda % 8))
       return fail(BFP8_EINVAL, "a must be row-major with 16-byte aligned rows");
   } else if (int r = check_codes(p.a, p.lda, p.sa, p.M, p.K)) {
@@ -434,7 +448,7 @@ int64_t bfp8_moe_workspace_bytes(const bfp8_moe_problem* pp) {
   const bfp8_moe_problem& p = *pp;
   if (int r = check_moe(p)) return r;
   MoeShape s;
-  if (!moe_shape(p, &s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
+  if (int r = moe_shape(p, &s)) return r;
   const int64_t pairs = int64_t(p.T) * p.top_k;
   return align256(pairs * p.I * 4) + align256(pairs * s.down.segments * p.H * 4) + align256(pairs * 8);
 }
@@ -445,7 +459,7 @@ int bfp8_launch_moe(const bfp8_moe_problem* pp, void* workspace, void* stream) {
   if (int r = check_moe(p)) return r;
   if (!workspace || !aligned16(workspace)) return fail(BFP8_EINVAL, "the workspace must be 16-byte aligned");
   MoeShape s;
-  if (!moe_shape(p, &s)) return fail(BFP8_EINVAL, "this expert layer's activations do not fit shared memory");
+  if (int r = moe_shape(p, &s)) return r;
   int dev = 0;
   const int num_sms = current_device_sms(&dev);
   if (num_sms < 0) return fail(BFP8_ECUDA, "no CUDA device");

@@ -343,8 +343,8 @@ int bfp8_launch_mxfp4_gemm(const bfp8_mxfp4_gemm_problem* p, void* stream);
  * w13 [E, 2 I, H] holds W1 (gate) over W3 (up); w2 [E, H, I].  format 0: block
  * FP8 (e4m3, scales fp32 [E, ceil(rows/128), ceil(K/128)]); 1: MXFP4 (codes
  * [E, rows, K/2], scale tiles [E, ceil(rows/128), ceil(K/128), 32, 16]).
- * 1 <= T <= 64, H and I multiples of 32, 32 <= H <= 8192, E <= 512, top_k <=
- * min(16, E).  Rows of x, y, w13 and w2 are 16-byte aligned. */
+ * 1 <= T <= 64, H and I multiples of 32, 32 <= H <= 8192, I <= 2^24, E <= 512,
+ * top_k <= min(16, E), T top_k max(I / 8, H I / 32768) below 2^31.  Rows of x, y, w13 and w2 are 16-byte aligned. */
 typedef struct bfp8_moe_problem {
   const void* x;
   int64_t ldx;

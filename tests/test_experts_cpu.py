@@ -189,3 +189,38 @@ def test_every_allowed_layer_has_a_layout(fmt):
                 for m.E in (1, 4, 128, 512):
                     for m.top_k in {1, min(8, m.E), min(16, m.E)}:
                         assert lib.bfp8_moe_workspace_bytes(ctypes.byref(m)) > 0, (m.T, m.H, m.I, m.E, m.top_k)
+
+
+@needs_native
+def test_c_abi_refuses_sizes_past_its_integers():
+    """Sizes whose tile and unit counts would leave 32 bits are refused with a reason, before any launch."""
+    lib = _native.capi()
+    big = 2 ** 31 - 32  # (K + 127) / 128 would overflow
+    q = _native.Mxfp4QuantProblem(x=16, ldx=big, x_type=1, q=16, ldq=big // 2, s=16, M=4, K=big)
+    assert lib.bfp8_launch_mxfp4_quantize(ctypes.byref(q), None) == _native.BFP8_EINVAL
+    q = _native.Mxfp4QuantProblem(x=16, ldx=64, x_type=1, q=16, ldq=32, s=16, M=2 ** 31 - 1, K=64)
+    assert lib.bfp8_launch_mxfp4_quantize(ctypes.byref(q), None) == _native.BFP8_EINVAL
+    d = _native.Mxfp4DequantProblem(q=16, ldq=big // 2, s=16, y=16, ldy=big, y_type=1, M=4, K=big)
+    assert lib.bfp8_launch_mxfp4_dequantize(ctypes.byref(d), None) == _native.BFP8_EINVAL
+    for sizes in ({"K": big}, {"M": 2 ** 31 - 1}, {"N": 2 ** 31 - 8}):
+        g = _native.Mxfp4GemmProblem(a=16, lda=big // 2, sa=16, b=16, ldb=big // 2, sb=16, c=16, ldc=2 ** 31, M=4, N=8, K=64)
+        for name, value in sizes.items():
+            setattr(g, name, value)
+        assert lib.bfp8_launch_mxfp4_gemm(ctypes.byref(g), None) == _native.BFP8_EINVAL, sizes
+    g = _native.Mxfp4GemmProblem(a=16, lda=big, b=16, ldb=big // 2, sb=16, c=16, ldc=8, M=4, N=8, K=big, a_type=1)
+    assert lib.bfp8_launch_mxfp4_gemm(ctypes.byref(g), None) == _native.BFP8_EINVAL
+
+    def layer(**sizes):
+        m = _native.MoeProblem(x=16, ldx=32, x_type=1, logits=16, ld_logits=16, logits_type=0, format=0, w13=16,
+                               w13_expert=1 << 40, w13_row=32, s13=16, w2=16, w2_expert=1 << 40, w2_row=1 << 32, s2=16,
+                               y=16, ldy=32, T=1, H=32, I=64, E=16, top_k=1)
+        for name, value in sizes.items():
+            setattr(m, name, value)
+        return lib.bfp8_moe_workspace_bytes(ctypes.byref(m))
+
+    assert layer() > 0 and layer(I=1 << 24) > 0
+    assert layer(I=(1 << 24) + 32) == _native.BFP8_EINVAL
+    assert layer(I=1 << 30) == _native.BFP8_EINVAL  # 2 I leaves 32 bits
+    # 64 x 16 pairs in chunks of their own: as many units as 2^31
+    assert layer(I=1 << 24, T=64, top_k=16) == _native.BFP8_EINVAL
+    assert b"units" in lib.bfp8_last_error()
