@@ -345,6 +345,11 @@ std::tuple<at::Tensor, at::Tensor> silu_mul_quant(const at::Tensor& x, double ep
 
 #define CHECK_VALUE(cond, ...) TORCH_CHECK_VALUE(cond, __VA_ARGS__)
 
+void require_valid(int status) {
+  CHECK_VALUE(status != BFP8_EINVAL, bfp8_last_error());
+  require_abi(status);
+}
+
 int float_type(const at::Tensor& t) {
   switch (t.scalar_type()) {
     case at::kFloat: return 0;
@@ -401,7 +406,7 @@ void check_mxfp4_input(const at::Tensor& x, const char* op) {
 void launch_mxfp4_quantize(const at::Tensor& x, const at::Tensor& q, const at::Tensor& s, bool trigger) {
   const bfp8_mxfp4_quant_problem p{x.data_ptr(),  row_stride(x), float_type(x),  q.data_ptr(),
                                    row_stride(q), s.data_ptr(),  int(x.size(0)), int(x.size(1)), trigger ? 1 : 0};
-  require_abi(bfp8_launch_mxfp4_quantize(&p, at::cuda::getCurrentCUDAStream().stream()));
+  require_valid(bfp8_launch_mxfp4_quantize(&p, at::cuda::getCurrentCUDAStream().stream()));
 }
 
 // x [M, K] -> (codes [M, K / 2], scale tiles).
@@ -426,7 +431,7 @@ at::Tensor dequantize_mxfp4(const at::Tensor& q, const at::Tensor& s, at::Scalar
   if (y.size(0) == 0) return y;
   const bfp8_mxfp4_dequant_problem p{q.data_ptr(), row_stride(q),  s.data_ptr(), y.data_ptr(), y.stride(0),
                                      float_type(y), int(y.size(0)), int(y.size(1))};
-  require_abi(bfp8_launch_mxfp4_dequantize(&p, at::cuda::getCurrentCUDAStream().stream()));
+  require_valid(bfp8_launch_mxfp4_dequantize(&p, at::cuda::getCurrentCUDAStream().stream()));
   return y;
 }
 
@@ -439,7 +444,7 @@ at::Tensor launch_mxfp4_gemm(const at::Tensor& a, const at::Tensor* sa, const at
                                   b.data_ptr(),   row_stride(b),  sb.data_ptr(),      c.data_ptr(),
                                   c.stride(0),    int(a.size(0)), int(b.size(0)),     int(2 * b.size(1)),
                                   weights_ready ? 1 : 0, sa ? 0 : float_type(a)};
-  require_abi(bfp8_launch_mxfp4_gemm(&p, at::cuda::getCurrentCUDAStream().stream()));
+  require_valid(bfp8_launch_mxfp4_gemm(&p, at::cuda::getCurrentCUDAStream().stream()));
   return c;
 }
 
@@ -548,9 +553,9 @@ at::Tensor launch_moe(const char* op, const at::Tensor& x, const at::Tensor& w13
   p.E = int(E);
   p.top_k = int(top_k);
   const int64_t bytes = bfp8_moe_workspace_bytes(&p);
-  require_abi(int(std::min<int64_t>(bytes, 0)));
+  require_valid(int(std::min<int64_t>(bytes, 0)));
   const at::Tensor ws = at::empty({bytes}, x.options().dtype(at::kByte));
-  require_abi(bfp8_launch_moe(&p, ws.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
+  require_valid(bfp8_launch_moe(&p, ws.data_ptr(), at::cuda::getCurrentCUDAStream().stream()));
   return y;
 }
 
