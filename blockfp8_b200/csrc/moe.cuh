@@ -12,12 +12,13 @@
 // counts, so the kernels are built to stream them:
 //
 // Measured (B200, device time of a call in a graph): 64 tokens, 128 experts, top
-// 8, H = 4096, I = 1280 in block FP8: 342 us for 2.0 GB of weights, 0.9 of the
-// measured copy rate; 13 tokens, 64 experts, top 6, I = 1408: 131 us; one token,
-// 128 experts, top 8, H = 2048, I = 768: 26 us for 38 MB (6 us at that rate):
-// there the router (3 us), the hand-over between the kernels and their ends
-// count, not the stream.  MXFP4, 40 tokens, 64 experts, top 4, I = 2048: 170 us
-// for 0.8 GB.
+// 8, H = 4096, I = 1280 in block FP8: 350 to 380 us for the 1.5 to 1.6 GB of the 96 to 104
+// experts that they meet; 13 tokens, 64 experts, top 6, I = 1408: 125 to 132 us for 37 to 43
+// of them; one token, 128 experts, top 8, H = 2048, I = 768: 27 us for 38 MB (6 us
+// at the measured copy rate): there the router (3 us), the hand-over between the
+// kernels and their ends count, not the stream.  MXFP4, 40 tokens, 64 experts, top
+// 4, I = 2048: 188 to 191 us for 0.6 GB.  (Batches run into the power limit: 1.7 to
+// 1.9 GHz; the lower figures are the first calls'.)
 //
 // - Work: (token, expert) pairs are grouped by expert into chunks of up to
 //   8, in token order (busier experts are read again, mostly from L2: chunks of 16
@@ -47,8 +48,8 @@
 //   at worst 2^-39 of the largest.  Up to four pairs have their upper parts in
 //   the MMA's columns 0-3 and the lower ones in 4-7.  Batches beyond 8 tokens have
 //   chunks of up to eight, whose parts lie in two planes of eight columns and
-//   take MMAs of their own (and a unit of them about an eighth more time: the
-//   CTAs' shares of units count them as such).
+//   take MMAs of their own (and a unit of them more time: the CTAs' shares count
+//   it a quarter more).
 // - A last warp finishes units: it adds the consumers' sums in warp order.
 //   z goes to memory and a small third kernel adds each token's pairs in j
 //   order.  (Counting arrivals and letting the last unit of an output row tile
@@ -673,24 +674,26 @@ __global__ void __launch_bounds__(Cfg::THREADS, Cfg::CTAS_PER_SM) moe_kernel(con
   const int tiles = GATE ? p.I / 8 : p.H / 16, per_chunk = tiles * p.segments;
   const int K = GATE ? p.H : p.I;
   // CTA b of G has units [x b / G, x (b + 1) / G) of all x = chunks * per_chunk;
-  // with BUSY, places where a unit of five pairs or more counts 9 and others 8.
+  // with BUSY, places where a unit of five pairs or more counts 5 and others 4
+  // (DOWN of MXFP4, 40 tokens, 10 of 52 chunks busy: 79 us, with 9 : 8 84, with 6 : 4
+  // 81; block FP8 within 3% between 9 : 8 and 11 : 8).
   auto first_unit = [&](int b) {
     if constexpr (!Cfg::BUSY) {
       return int(int64_t(chunks) * per_chunk * b / gridDim.x);
     } else {
       auto busy_of = [&](int c) { return __ballot_sync(~0u, c < chunks && route.chunk_count[c] > kMoeBeside); };
-      int total = 8 * chunks;
+      int total = 4 * chunks;
       for (int c = 0; c < chunks; c += 32) total += __popc(busy_of(c + lane));
       const int64_t place = int64_t(total) * per_chunk * b / gridDim.x;
       int64_t before = 0;
       for (int c = 0; c < chunks; c += 32) {
         const uint32_t busy = busy_of(c + lane);
-        const int n = min(32, chunks - c), own = busy >> lane & 1u ? 9 : 8;
-        const int64_t at = before + int64_t(8 * lane + __popc(busy & ((1u << lane) - 1u))) * per_chunk;
+        const int n = min(32, chunks - c), own = busy >> lane & 1u ? 5 : 4;
+        const int64_t at = before + int64_t(4 * lane + __popc(busy & ((1u << lane) - 1u))) * per_chunk;
         const uint32_t mine = __ballot_sync(~0u, lane < n && place >= at && place < at + int64_t(own) * per_chunk);
         const int u = (c + lane) * per_chunk + int((place - at) / own);
         if (mine) return __shfl_sync(~0u, u, __ffs(mine) - 1);
-        before += int64_t(8 * n + __popc(busy)) * per_chunk;
+        before += int64_t(4 * n + __popc(busy)) * per_chunk;
       }
       return chunks * per_chunk;
     }
