@@ -12,13 +12,13 @@
 // counts, so the kernels are built to stream them:
 //
 // Measured (B200, device time of a call in a graph): 64 tokens, 128 experts, top
-// 8, H = 4096, I = 1280 in block FP8: 350 to 380 us for the 1.5 to 1.6 GB of the 96 to 104
-// experts that they meet; 13 tokens, 64 experts, top 6, I = 1408: 125 to 132 us for 37 to 43
-// of them; one token, 128 experts, top 8, H = 2048, I = 768: 27 us for 38 MB (6 us
-// at the measured copy rate): there the router (3 us), the hand-over between the
-// kernels and their ends count, not the stream.  MXFP4, 40 tokens, 64 experts, top
-// 4, I = 2048: 188 to 191 us for 0.6 GB.  (Batches run into the power limit: 1.7 to
-// 1.9 GHz; the lower figures are the first calls'.)
+// 8, H = 4096, I = 1280 in block FP8: 350 to 380 us for the 1.5 to 1.6 GB of the
+// 96 to 104 experts that they meet; 13 tokens, 64 experts, top 6, I = 1408: 125 to
+// 132 us for 37 to 43 of them; one token, 128 experts, top 8, H = 2048, I = 768: 27
+// us for 38 MB (6 us at the measured copy rate): there the router (3 us), the
+// hand-over between the kernels and their ends count, not the stream.  MXFP4, 40
+// tokens, 64 experts, top 4, I = 2048: 188 to 191 us for 0.6 GB.  (Batches run into
+// the power limit: 1.7 to 1.9 GHz; the lower figures are the first calls'.)
 //
 // - Work: (token, expert) pairs are grouped by expert into chunks of up to
 //   8, in token order (busier experts are read again, mostly from L2: chunks of 16

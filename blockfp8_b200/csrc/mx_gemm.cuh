@@ -330,10 +330,9 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
 // A cluster of two CTAs computes 256 tokens x 256 weight rows with
 // cta_group::2 MMAs (M = 256, N = 256, K = 64): each CTA holds 128 token rows
 // and 128 of the weight rows, so a stage of K = 256 costs an SM 35 KB of
-// shared-memory fill for 512 clocks of MMA (70 B per clock; the L2 delivers
-// about 62 to every SM at once, which is this kernel's bound, ahead of the
-// tensor cores).  Token rows are the MMA rows: a thread of the epilogue holds
-// one row's consecutive columns.
+// shared-memory fill for 512 clocks of MMA (70 B per clock while MMAs run).  Token
+// rows are the MMA rows: a thread of the epilogue holds one row's consecutive
+// columns.
 //
 // TMEM: 256 accumulator columns and every stage's scales (each CTA its token
 // rows', and all 256 weight rows').
@@ -345,8 +344,13 @@ __global__ void __launch_bounds__(Cfg::THREADS) mx_gemm_kernel(const __grid_cons
 // tiles share operands in L2.
 //
 // Measured: 8192 x 24576 x 4096 in 322 us (5.1 PFLOP/s; the MMAs alone, without
-// loads, 231 us).  One thread that issues everything is what held it back: 507 us
-// with the scales' copies in the MMA thread, 340 with a thread of their own.
+// loads, 231 us).  Over the whole kernel the tensor pipe is busy for 0.66 of the
+// clocks, an SM receives 44 B per clock and L2 is at 0.47 of its peak: what is left
+// is loads that come late to the K loop and the epilogue between tiles.  One thread
+// that issues everything is what held it back: 507 us with the scales' copies in
+// the MMA thread, 340 with a thread of their own.  That is at 1.6 GHz or more;
+// calls without a pause run into the power limit, at 1.45 to 1.5 GHz and 405 to
+// 415 us, from a graph as from Python.
 //
 // Warps: TMA producers 0 (weights), 12 (tokens) and 2 (scales), 1 MMA issuer and
 // TMEM owner, 3 issuer of the scales' copies into TMEM (1 and 3 the leader's),

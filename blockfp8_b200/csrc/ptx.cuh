@@ -1,7 +1,8 @@
 // sm_100a primitives used by the kernels: mbarriers with bounded waits, TMA
 // tile loads and stores, and the tcgen05 (5th-generation tensor core) MMA,
-// commit, TMEM allocation and TMEM loads.  Hand-written inline PTX; no
-// cluster multicast anywhere (these kernels also run on multi-GPU jobs).
+// commit, TMEM allocation and TMEM loads.  Hand-written inline PTX; no load
+// with cluster multicast anywhere (these kernels also run on multi-GPU jobs;
+// mma_commit_pair's multicast is an arrival on two barriers).
 #pragma once
 
 #include <cuda.h>

@@ -15,8 +15,10 @@ which holds bf16 exactly down to 2^-28 of the largest of them; h as two such
 parts, 22 bits of each value (2^-39 of the largest at worst).  (The dense
 block-FP8 linear quantizes its activations; a layer built from it differs by
 that rounding.)
-Two kernels and no synchronisation; results do not depend on the order in
-which CTAs finish.  H and I are multiples of 32, H at most 8192, E at most
+Three launches (two kernels that stream weights, and a small sum) and no
+synchronisation; results do not depend on the order in which CTAs finish.
+MXFP4 scales multiply fp32 sums before the activations' own powers of two do:
+scale bytes above 230 (2^103) may overflow there although the result would not.  H and I are multiples of 32, H at most 8192, E at most
 512, top_k at most 16.  The kernels check their arguments themselves
 (ValueError).  No reference counterpart: the reference covers dense linears.
 """

@@ -50,7 +50,9 @@ def quantize_mxfp4(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def dequantize_mxfp4(q: torch.Tensor, scales: torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
-    """The values that the codes stand for, [M, K] bfloat16 or float32 (exact in both)."""
+    """The values that the codes stand for, [M, K] bfloat16 or float32.  Exact in both for what quantize_mxfp4
+    makes (scale bytes up to 252); under the bytes 253 and 254 codes of 4 and 6 (254: 2 and more) are infinite in
+    both types."""
     return ops.dequantize_mxfp4(q, scales, dtype=dtype)
 
 
