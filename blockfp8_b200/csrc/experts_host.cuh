@@ -182,7 +182,10 @@ bool moe_layout(const bfp8_moe_problem& p, int k, int segments, int entries, boo
   out->unit_stages = unit_stages;
   out->seg_len = segments == 1 ? columns * per_column : unit_stages * out->box * per_column;
   out->segments = cdiv(k, out->seg_len);
-  out->resident = entries <= kMoeChunk && (!down || warps == 8);
+  // (DOWN's second four pairs take a plane of their own: beyond 64 KB that costs
+  // the ring more than laying out each chunk's pairs: MXFP4, 2 tokens, 64 experts,
+  // top 4, H = I = 2880: 55 us against 47.)
+  out->resident = entries <= kMoeChunk && (!down || (warps == 8 && (entries <= kMoeBeside || k <= kMoeBusySegment)));
   out->cols = down ? (out->resident ? 2 * std::min(entries, kMoeBeside) : kMoeChunk)
                    : out->resident ? entries : std::min(P, kMoeChunk);
   const int planes = !down ? 1 : out->resident ? cdiv(entries, kMoeBeside) : warps == 8 ? 1 : 2;
@@ -216,8 +219,7 @@ struct MoeShape {
 };
 
 bool moe_layouts(const bfp8_moe_problem& p, MoeShape* s) {
-  const int P = p.T * p.top_k, busy = cdiv(p.I, kMoeBusySegment);
-  const int few = P > kMoeBeside && P <= kMoeChunk ? busy : cdiv(p.I, kMoeSegment);
+  const int P = p.T * p.top_k;
   auto one = [&](int k, int ranges, int entries, bool down, int warps, int limit, MoeLayout* lay) {
     s->warps = warps;
     for (int box = 8; box >= 1; box /= 2)
@@ -228,9 +230,9 @@ bool moe_layouts(const bfp8_moe_problem& p, MoeShape* s) {
   // leaves, so that DOWN starts beside GATE and requests its weights while GATE
   // runs.
   if (p.T <= 8 && one(p.H, 1, p.T, false, 8, kMoeHalfSmem, &s->gate) &&
-      one(p.I, few, P, true, 8, kMoeSharedSmem - s->gate.smem, &s->down))
+      one(p.I, cdiv(p.I, kMoeSegment), P, true, 8, kMoeSharedSmem - s->gate.smem, &s->down))
     return true;
-  return one(p.H, 1, p.T, false, 16, kMaxSmem, &s->gate) && one(p.I, busy, P, true, 16, kMaxSmem, &s->down);
+  return one(p.H, 1, p.T, false, 16, kMaxSmem, &s->gate) && one(p.I, cdiv(p.I, kMoeBusySegment), P, true, 16, kMaxSmem, &s->down);
 }
 
 int moe_shape(const bfp8_moe_problem& p, MoeShape* s) {
